@@ -26,6 +26,7 @@ GKV_F32, GKV_F16, GKV_BF16 = 0, 1, 30
 GKV_KV_BF16, GKV_KV_FP8_E4M3 = 0, 1  # gkv_kv_format
 
 i32 = C.c_int32
+i64 = C.c_int64
 vp = C.c_void_p
 i32p = C.POINTER(C.c_int32)
 u32p = C.POINTER(C.c_uint32)
@@ -49,6 +50,31 @@ class NewPages(C.Structure):
 class QkNormDesc(C.Structure):
     _fields_ = [("q_norm_w", vp), ("k_norm_w", vp), ("cos_tab", vp), ("sin_tab", vp), ("max_seq", i32),
                 ("eps", C.c_float)]
+
+
+class Batch(C.Structure):
+    _fields_ = [("pool", PoolDesc), ("table", vp), ("lens", vp), ("table_stride", i64), ("batch", i32),
+                ("table_pages", i32), ("device", i32)]
+
+
+class BatchDecodeArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_stride_batch", i64), ("q_stride_head", i64), ("k_new", vp), ("v_new", vp),
+                ("k_stride_batch", i64), ("k_stride_head", i64), ("v_stride_batch", i64), ("v_stride_head", i64),
+                ("out", vp), ("lse", vp), ("pages", vp), ("weights_in", vp), ("weights_out", vp),
+                ("weights_stride", i64), ("n_pages", i32), ("n_q_heads", i32), ("out_dtype", i32),
+                ("scale", C.c_float), ("decay", C.c_float), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class BatchSelectArgs(C.Structure):
+    _fields_ = [("q", vp), ("q_stride_batch", i64), ("q_stride_head", i64), ("bounds", vp), ("pages", vp),
+                ("n_pages", i32), ("n_first", i32), ("n_last", i32), ("extra", i32), ("n_q_heads", i32),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class BatchEvictArgs(C.Structure):
+    _fields_ = [("weights", vp), ("weights_out", vp), ("positions", vp), ("positions_out", vp), ("seen", vp),
+                ("tracked", vp), ("lens_out", vp), ("stride", i64), ("n_keep", i32), ("n_recent", i32),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
 
 
 # name -> (argtypes, restype); every entry point returns an int status unless noted.
@@ -117,6 +143,15 @@ SIGNATURES = {
                                         C.c_float, i32, i32, C.POINTER(QkNormDesc), vp], C.c_int),
     "gkv_paged_attention_qknorm": ([vp, i32, vp, vp, vp, vp, i32, i32, C.c_float, i32, i32, C.POINTER(QkNormDesc),
                                     vp], C.c_int),
+    "gkv_batch_prepare": ([C.c_int], C.c_int),
+    "gkv_batch_check_errors": ([C.c_int, u32p], C.c_int),
+    "gkv_batch_decode_workspace": ([C.POINTER(Batch), i32, i32, C.POINTER(C.c_size_t)], C.c_int),
+    "gkv_batch_decode": ([C.POINTER(Batch), C.POINTER(BatchDecodeArgs), vp], C.c_int),
+    "gkv_batch_page_bounds": ([C.POINTER(Batch), vp, i32, vp, vp], C.c_int),
+    "gkv_batch_select_workspace": ([C.POINTER(Batch), C.POINTER(C.c_size_t)], C.c_int),
+    "gkv_batch_select_pages": ([C.POINTER(Batch), C.POINTER(BatchSelectArgs), vp], C.c_int),
+    "gkv_batch_evict_workspace": ([C.POINTER(Batch), C.POINTER(C.c_size_t)], C.c_int),
+    "gkv_batch_evict": ([C.POINTER(Batch), C.POINTER(BatchEvictArgs), vp], C.c_int),
 }
 
 

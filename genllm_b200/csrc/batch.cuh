@@ -1,0 +1,87 @@
+// batch.cuh — device helpers shared by the batch tier's kernels.
+#pragma once
+#include "batch.h"
+#include "device.cuh"
+
+namespace gkv {
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Pages that hold n tokens, at most the table row's.
+__device__ __forceinline__ int pages_of(int n) { return (n + kPageSlots - 1) / kPageSlots; }
+
+// base[b] = sum of count(b') over b' < b, for b = 0 .. batch: every thread of
+// the CTA calls it; base and warp_sums (32 ints) are shared memory. A thread
+// sums a run of consecutive sequences, so one pass serves any batch.
+template <typename Count>
+__device__ __forceinline__ void scan_counts(int batch, int* base, int* warp_sums, Count count) {
+    const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31;
+    const int run = (batch + n - 1) / n;
+    const int b0 = min(batch, tid * run), b1 = min(batch, b0 + run);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+        const int c = count(b);
+        base[b] = c;
+        sum += c;
+    }
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 31) warp_sums[tid >> 5] = inc;
+    __syncthreads();
+    int before = inc - sum;
+    for (int w = 0; w < (tid >> 5); ++w) before += warp_sums[w];
+    for (int b = b0; b < b1; ++b) {
+        const int c = base[b];
+        base[b] = before;
+        before += c;
+    }
+    if (tid == n - 1) base[batch] = before;
+    __syncthreads();
+}
+
+// The sequence that owns unit u: the last b with base[b] * per <= u.
+__device__ __forceinline__ int owner(const int* base, int batch, int per, int u) {
+    int lo = 0, hi = batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (base[mid] * per <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
+                 "l"(policy)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Launch as a programmatic dependent: the kernel waits (pdl_wait) before it
+// touches anything the kernels ahead of it on the stream write.
+template <typename... Args, typename... Given>
+inline cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                    Given... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args>(args)...);
+}
+
+}  // namespace gkv

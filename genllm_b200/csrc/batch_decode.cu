@@ -1,0 +1,628 @@
+// batch_decode.cu — attention of one new token for each of many sequences over
+// a paged cache, split over the pages and joined.
+//
+// For sequence b and query head q of kv head h, over the attended tokens t:
+//   s_t = scale * q.k_t,  out = sum_t exp(s_t - lse) v_t,  lse = ln sum_t exp(s_t),
+// in one pass over K and V with the running maximum and sum (fp32, in log2
+// units); a sequence cut into several parts leaves (maximum, sum, un-normalised
+// output) of each part in the workspace, joined in order by the second kernel.
+//
+// Work: the pages of all sequences form one line of units (x head groups); a
+// worker takes an equal, contiguous part of it, whatever the lengths are, so
+// ragged batches load every SM alike. It has at most two parts that other
+// workers continue (its first and its last); what lies between it finishes
+// itself. Bound: HBM (K and V once); a worker is one warp per kv head of a
+// group, so that a page's [16][Hkv][D] bytes are read together.
+//
+// One unit is 16 keys of one head: S^T = K Q^T (M 16 keys, N 8 query heads)
+// and O^T += V^T P^T (M 16 dims) on mma.sync, the keys' rows coming through a
+// per-warp cp.async ring, 16-byte chunks XOR-permuted by row for ldmatrix.
+// mma.sync and not tcgen05: at 16 query heads or fewer the products are far
+// below the stream of K and V in cost, and each warp works without barriers.
+#include "batch.cuh"
+
+namespace gkv {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr int kMinUnits = 4;  // pages of a worker at least: below that the join costs more than it spreads
+constexpr int kRingBytes = 192 * 1024;
+
+struct DecodeParams {
+    BatchView v;
+    BatchDecodeLaunch d;
+    BatchSplit s;
+    int32_t group;       // query heads per kv head
+    int32_t min_units;
+    float scale_log2;
+    float* part_acc;     // [2 workers][heads * group][D]
+    float2* part_ml;     // [2 workers][heads * group] (maximum in log2 units, sum)
+    float* lse2;         // [batch][Hq] log2 of the sum, for the totals
+    int32_t* base;       // [batch + 1] units before each sequence
+    float* scores;       // [unit][16][group] scores in log2 units, for the totals; or null
+};
+
+__device__ __forceinline__ float exp2_of(float x) { return exp2_approx(x); }
+
+// Tokens sequence b attends (with the new one), 0 for a skipped sequence;
+// flags a length its table row cannot hold and leaves out what lies behind.
+__device__ __forceinline__ int attended(const BatchView& v, const BatchDecodeLaunch& d, int b, bool flag) {
+    const int len = v.lens[b];
+    if (len < 0) return 0;
+    const int cap = v.table_pages * kPageSlots;
+    const int new_token = d.k_new ? 1 : 0;
+    if (len > cap - new_token) {
+        if (flag) atomicOr(v.err, kErrBadLength);
+        return cap;
+    }
+    return len + new_token;
+}
+
+// Whether sequence b gains a token this step, and where.
+__device__ __forceinline__ bool gains(const BatchView& v, const BatchDecodeLaunch& d, int b, int* pos) {
+    const int len = v.lens[b];
+    *pos = len;
+    return d.k_new && len >= 0 && len < v.table_pages * kPageSlots;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <bool F16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if (F16) return __half22float2(*reinterpret_cast<__half2*>(&w));
+    return make_float2(bf16_lo(w), bf16_hi(w));
+}
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+// What a lane holds of one unit ahead of its loads.
+struct Unit {
+    int k_id, v_id;
+    int info;  // valid rows | kNewRow: the last of them is the new token
+    int bh;    // sequence * hkv + head
+};
+constexpr int kNewRow = 1 << 8;
+
+template <bool F16, int D, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const DecodeParams p) {
+    constexpr int kRow = D * 2;              // bytes of one head's row
+    constexpr int kTile = kPageSlots * kRow;  // one unit's K (or V)
+    constexpr int kStages = kRingBytes / (WARPS * 2 * kTile);
+    constexpr int kChunks = kRow / 16;       // 16-byte chunks of a row
+    constexpr int kRowsPerCopy = 32 / kChunks;
+    constexpr int kCopies = kPageSlots / kRowsPerCopy;
+    constexpr int kSteps = D / 16;
+    static_assert(kStages >= 2, "the ring holds one unit ahead");
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int warp_sums[32];
+    __shared__ int stage_info[WARPS][kStages];
+    int* base = reinterpret_cast<int*>(smem + kRingBytes);
+
+    const BatchView& v = p.v;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_trigger();
+    pdl_wait();
+
+    const int n_list = p.d.pages ? p.d.n_pages : 0x7FFFFFFF;
+    scan_counts(v.batch, base, warp_sums,
+                [&](int b) { return min(n_list, pages_of(attended(v, p.d, b, blockIdx.x == 0))); });
+    const int total = base[v.batch] * p.s.groups;
+    const int per = max(p.min_units, (total + p.s.workers - 1) / p.s.workers);
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= v.batch; b += blockDim.x) p.base[b] = base[b];
+
+    const int hq = p.d.n_q_heads;
+    for (int b = blockIdx.x; b < v.batch; b += gridDim.x) {
+        // The new token's rows go to their page slot; its readers below take
+        // them from the step's inputs, so neither waits for the other.
+        int pos;
+        if (gains(v, p.d, b, &pos)) {
+            const int2 e = v.table[b * v.table_stride + pos / kPageSlots];
+            const bool ok = e.x >= 0 && e.x < v.pool_pages && e.y >= 0 && e.y < v.pool_pages;
+            if (!ok && tid == 0) atomicOr(v.err, kErrBadPage);
+            for (int i = tid; ok && i < 2 * v.hkv * kChunks; i += blockDim.x) {
+                const bool is_v = i >= v.hkv * kChunks;
+                const int j = is_v ? i - v.hkv * kChunks : i, h = j / kChunks, c = j % kChunks;
+                const uint16_t* src = is_v ? p.d.v_new + b * p.d.v_stride_batch + h * p.d.v_stride_head
+                                           : p.d.k_new + b * p.d.k_stride_batch + h * p.d.k_stride_head;
+                uint16_t* dst = (is_v ? v.v_base : v.k_base) +
+                                (((size_t)(is_v ? e.y : e.x) * kPageSlots + pos % kPageSlots) * v.hkv + h) * D;
+                reinterpret_cast<uint4*>(dst)[c] = reinterpret_cast<const uint4*>(src)[c];
+            }
+        }
+        // Nothing to attend: zeros (a skipped sequence is left alone).
+        if (v.lens[b] >= 0 && base[b + 1] == base[b]) {
+            for (int i = tid; i < hq * D; i += blockDim.x) store_out(p.d.out, (size_t)b * hq * D + i, 0.f, p.d.out_dtype);
+            for (int i = tid; i < hq; i += blockDim.x) {
+                if (p.d.lse) p.d.lse[(size_t)b * hq + i] = -INFINITY;
+                p.lse2[(size_t)b * hq + i] = -INFINITY;
+            }
+        }
+    }
+
+    const int worker = blockIdx.x * p.s.lanes + warp / p.s.heads;
+    const int head_in = warp % p.s.heads;
+    if (warp >= p.s.lanes * p.s.heads) return;
+    const int64_t first = (int64_t)worker * per;
+    if (first >= total) return;
+    const int u0 = (int)first, u1 = (int)min((int64_t)total, first + per);
+
+    const uint64_t policy = l2_policy_evict_first();
+    uint8_t* ring = smem + warp * (kStages * 2 * kTile);
+    const uint32_t ring_addr = smem_addr(ring);
+    const size_t slot_stride = (size_t)v.hkv * D;
+
+    // This lane's unit of the 32 from `from` on.
+    auto fetch = [&](int from) {
+        Unit n{0, 0, 0, 0};
+        const int u = from + lane;
+        if (u >= u1) return n;
+        const int b = owner(base, v.batch, p.s.groups, u);
+        const int count = base[b + 1] - base[b];
+        const int r = u - base[b] * p.s.groups;
+        const int grp = r / count, j = r - grp * count;
+        const int h = grp * p.s.heads + head_in;
+        if (h >= v.hkv) return n;
+        const int tokens = attended(v, p.d, b, false);
+        n.bh = b * v.hkv + h;
+        const int lp = p.d.pages ? p.d.pages[(size_t)n.bh * p.d.n_pages + j] : j;
+        if (lp < 0 || lp >= pages_of(tokens)) return n;
+        const int2 e = v.table[b * v.table_stride + lp];
+        if (e.x < 0 || e.x >= v.pool_pages || e.y < 0 || e.y >= v.pool_pages) {
+            atomicOr(v.err, kErrBadPage);
+            return n;
+        }
+        n.k_id = e.x;
+        n.v_id = e.y;
+        n.info = min(kPageSlots, tokens - lp * kPageSlots);
+        int pos;
+        if (gains(v, p.d, b, &pos) && pos / kPageSlots == lp) n.info |= kNewRow;
+        return n;
+    };
+
+    Unit cur = fetch(u0), next = fetch(u0 + 32);
+    int cur_from = u0;
+    const int c16 = lane % kChunks, r0 = lane / kChunks;
+
+    auto issue = [&](int u) {
+        if (u < u1) {
+            if (u - cur_from >= 32) {
+                cur = next;
+                cur_from += 32;
+                next = fetch(cur_from + 32);
+            }
+            const int from = u - cur_from;
+            const int k_id = __shfl_sync(0xFFFFFFFFu, cur.k_id, from), v_id = __shfl_sync(0xFFFFFFFFu, cur.v_id, from);
+            const int info = __shfl_sync(0xFFFFFFFFu, cur.info, from), bh = __shfl_sync(0xFFFFFFFFu, cur.bh, from);
+            const int h = bh % v.hkv, valid = info & 0xFF;
+            const int stage = (u - u0) % kStages;
+            if (lane == 0) stage_info[warp][stage] = valid;
+            const uint32_t dst = ring_addr + stage * (2 * kTile);
+            const uint16_t* k = v.k_base + ((size_t)k_id * kPageSlots + r0) * slot_stride + h * D + c16 * 8;
+            const uint16_t* vv = v.v_base + ((size_t)v_id * kPageSlots + r0) * slot_stride + h * D + c16 * 8;
+            const bool has_new = info & kNewRow;
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const int row = i * kRowsPerCopy + r0;
+                const uint32_t to = dst + row * kRow + ((c16 ^ (row & 7)) << 4);
+                const uint16_t* ks = k + i * kRowsPerCopy * slot_stride;
+                const uint16_t* vs = vv + i * kRowsPerCopy * slot_stride;
+                if (has_new && row == valid - 1) {
+                    const int b = bh / v.hkv;
+                    ks = p.d.k_new + b * p.d.k_stride_batch + h * p.d.k_stride_head + c16 * 8;
+                    vs = p.d.v_new + b * p.d.v_stride_batch + h * p.d.v_stride_head + c16 * 8;
+                }
+                // Rows behind the sequence become zeros: what the slots hold may be anything.
+                const uint32_t bytes = row < valid ? 16u : 0u;
+                cp_async16(to, ks, bytes, policy);
+                cp_async16(to + kTile, vs, bytes, policy);
+            }
+        }
+        cp_async_commit();
+    };
+
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
+
+    const int g4 = lane >> 2, c2 = (lane & 3) * 2;  // fragment row, first column
+    const int k_row = lane & 15, k_chunk = lane >> 4;
+    const int v_row = (lane & 7) + ((lane >> 4) << 3), v_chunk = (lane >> 3) & 1;
+    const int G = p.group;
+
+    int u = u0;
+    while (u < u1) {
+        // One segment: the rest of (sequence, head group) inside [u, u1).
+        const int b = owner(base, v.batch, p.s.groups, u);
+        const int count = base[b + 1] - base[b];
+        const int seq0 = base[b] * p.s.groups;
+        const int grp = (u - seq0) / count;
+        const int seg0 = seq0 + grp * count, seg1 = seg0 + count;
+        const int begin = u, end = min(u1, seg1);
+        const int h = grp * p.s.heads + head_in;
+        const bool mine = h < v.hkv;
+        float* score_row = p.scores && mine
+                               ? p.scores + ((size_t)base[b] * v.hkv + (size_t)h * count) * (kPageSlots * G)
+                               : nullptr;
+
+        // Q of the segment as B fragments (16 dims x 8 heads).
+        uint32_t qf[NT][kSteps][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int g = nt * 8 + g4;
+            const uint16_t* row = p.d.q + b * p.d.q_stride_batch + (int64_t)(h * G + g) * p.d.q_stride_head + c2;
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+                qf[nt][ks][0] = mine && g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
+                qf[nt][ks][1] = mine && g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
+            }
+        }
+        float acc[NT][kSteps][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+        }
+        bool any_key = false;
+
+        for (; u < end; ++u) {
+            cp_async_wait<kStages - 2>();
+            __syncwarp();
+            issue(u + kStages - 1);
+            const int stage = (u - u0) % kStages;
+            const int valid = stage_info[warp][stage];
+            if (valid == 0) {
+                // A skipped page gets no weight.
+                for (int i = lane; score_row && i < kPageSlots * G; i += 32)
+                    score_row[(size_t)(u - seg0) * (kPageSlots * G) + i] = -INFINITY;
+                continue;
+            }
+            any_key = true;
+            const uint32_t tile = ring_addr + stage * (2 * kTile);
+
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) {
+                uint32_t a[4];
+                ldmatrix4(a, tile + k_row * kRow + (((2 * ks + k_chunk) ^ (k_row & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<F16>(s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+            }
+            uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] *= p.scale_log2;
+                if (score_row) {
+                    float* at = score_row + (size_t)(u - seg0) * (kPageSlots * G) + g4 * G + nt * 8 + c2;
+                    const int left = G - nt * 8 - c2;
+                    if (left > 0) at[0] = s[nt][0], at[8 * G] = s[nt][2];
+                    if (left > 1) at[1] = s[nt][1], at[8 * G + 1] = s[nt][3];
+                }
+                if (valid < kPageSlots) {
+                    if (g4 >= valid) s[nt][0] = s[nt][1] = -INFINITY;
+                    if (g4 + 8 >= valid) s[nt][2] = s[nt][3] = -INFINITY;
+                }
+                float x0 = fmaxf(s[nt][0], s[nt][2]), x1 = fmaxf(s[nt][1], s[nt][3]);
+                // The maximum moves seldom once some pages are in.
+                if (__any_sync(0xFFFFFFFFu, x0 > m[nt][0] || x1 > m[nt][1])) {
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) {
+                        x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, o));
+                        x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, o));
+                    }
+                    const float n0 = fmaxf(m[nt][0], x0), n1 = fmaxf(m[nt][1], x1);
+                    const float a0 = n0 == m[nt][0] ? 1.f : exp2_of(m[nt][0] - n0);
+                    const float a1 = n1 == m[nt][1] ? 1.f : exp2_of(m[nt][1] - n1);
+                    m[nt][0] = n0;
+                    m[nt][1] = n1;
+                    l[nt][0] *= a0;
+                    l[nt][1] *= a1;
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        acc[nt][i][0] *= a0;
+                        acc[nt][i][1] *= a1;
+                        acc[nt][i][2] *= a0;
+                        acc[nt][i][3] *= a1;
+                    }
+                }
+                // Scores of -inf alone leave the maximum there: their weights are 0.
+                const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+                const float p0 = exp2_of(s[nt][0] - m0), p1 = exp2_of(s[nt][1] - m1);
+                const float p2 = exp2_of(s[nt][2] - m0), p3 = exp2_of(s[nt][3] - m1);
+                l[nt][0] += p0 + p2;
+                l[nt][1] += p1 + p3;
+                // P as two 16-bit terms, so that the product with V keeps more than
+                // 16 bits of each weight (one term would lose 2^-9 of it in bf16).
+                const uint32_t h01 = pack2<F16>(p0, p1), h23 = pack2<F16>(p2, p3);
+                const float2 r01 = unpack2<F16>(h01), r23 = unpack2<F16>(h23);
+                hi[nt][0] = transpose8x8(h01);
+                hi[nt][1] = transpose8x8(h23);
+                lo[nt][0] = transpose8x8(pack2<F16>(p0 - r01.x, p1 - r01.y));
+                lo[nt][1] = transpose8x8(pack2<F16>(p2 - r23.x, p3 - r23.y));
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                uint32_t a[4];
+                ldmatrix4_trans(a, tile + kTile + v_row * kRow + (((2 * i + v_chunk) ^ (v_row & 7)) << 4));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816<F16>(acc[nt][i], a, hi[nt][0], hi[nt][1]);
+                    mma16816<F16>(acc[nt][i], a, lo[nt][0], lo[nt][1]);
+                }
+            }
+        }
+        if (!mine) continue;
+
+        const bool whole = begin == seg0 && end == seg1;
+        const int rows = p.s.heads * G;
+        const size_t slot = (size_t)(2 * worker + (begin == u0 ? 0 : 1)) * rows + head_in * G;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][i], o);
+                const int g = nt * 8 + c2 + i;
+                if (g >= G) continue;
+                const size_t q_row = (size_t)b * hq + h * G + g;
+                if (whole) {
+                    const float inv = any_key ? 1.f / l[nt][i] : 0.f;
+                    if (g4 == 0) {
+                        const float e = any_key ? m[nt][i] + log2f(l[nt][i]) : -INFINITY;
+                        p.lse2[q_row] = e;
+                        if (p.d.lse) p.d.lse[q_row] = e * kLn2;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        store_out(p.d.out, q_row * D + k * 16 + g4, acc[nt][k][i] * inv, p.d.out_dtype);
+                        store_out(p.d.out, q_row * D + k * 16 + g4 + 8, acc[nt][k][i + 2] * inv, p.d.out_dtype);
+                    }
+                } else {
+                    // A part whose scores were all -inf is told from one without keys by its maximum.
+                    if (g4 == 0)
+                        p.part_ml[slot + g] =
+                            make_float2(any_key && m[nt][i] == -INFINITY ? kLowest : m[nt][i], l[nt][i]);
+                    float* to = p.part_acc + (slot + g) * D + g4;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) {
+                        to[k * 16] = acc[nt][k][i];
+                        to[k * 16 + 8] = acc[nt][k][i + 2];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Joins the parts of each cut sequence, in order: block (segment, row), the
+// row one of the group's query heads; eight warps take the parts in turn.
+constexpr int kJoinWarps = 8;
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) batch_join_kernel(const DecodeParams p) {
+    constexpr int kPer = D / 32;
+    __shared__ float sh_acc[kJoinWarps][D];
+    __shared__ float2 sh_ml[kJoinWarps];
+    pdl_wait();
+    pdl_trigger();
+    const int total = p.base[p.v.batch] * p.s.groups;
+    const int per = max(p.min_units, (total + p.s.workers - 1) / p.s.workers);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rows = p.s.heads * p.group;
+    for (int seg = blockIdx.x; seg < p.v.batch * p.s.groups; seg += gridDim.x) {
+        const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
+        const int count = p.base[b + 1] - p.base[b];
+        if (count == 0) continue;
+        const int s0 = p.base[b] * p.s.groups + grp * count, s1 = s0 + count;
+        const int w0 = s0 / per, w1 = (s1 - 1) / per;
+        if (w0 == w1) continue;
+        const int head = grp * p.s.heads + (int)blockIdx.y / p.group;
+        if (head >= p.v.hkv) continue;
+        float m = -INFINITY, l = 0.f, acc[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
+        for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
+            const size_t slot = (size_t)(2 * w + (w == w0 && s0 != w0 * per ? 1 : 0)) * rows + blockIdx.y;
+            const float2 ml = p.part_ml[slot];
+            const float n = fmaxf(m, ml.x);
+            const float a = n == m ? 1.f : exp2_of(m - n), c = n == ml.x ? 1.f : exp2_of(ml.x - n);
+            m = n;
+            l = l * a + ml.y * c;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * a + p.part_acc[slot * D + i * 32 + lane] * c;
+        }
+        if (lane == 0) sh_ml[warp] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sh_acc[warp][i * 32 + lane] = acc[i];
+        __syncthreads();
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) M = fmaxf(M, sh_ml[w].x);
+        float c[kJoinWarps];
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+            c[w] = sh_ml[w].x == M ? 1.f : exp2_of(sh_ml[w].x - M);
+            L += sh_ml[w].y * c[w];
+        }
+        const size_t q_row = (size_t)b * p.d.n_q_heads + grp * rows + blockIdx.y;
+        const bool none = M == -INFINITY;  // no key at all
+        const float inv = none ? 0.f : 1.f / L;
+        for (int d = threadIdx.x; d < D; d += blockDim.x) {
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) o += sh_acc[w][d] * c[w];
+            store_out(p.d.out, q_row * D + d, o * inv, p.d.out_dtype);
+        }
+        if (threadIdx.x == 0) {
+            const float e = none ? -INFINITY : M + log2f(L);
+            p.lse2[q_row] = e;
+            if (p.d.lse) p.d.lse[q_row] = e * kLn2;
+        }
+        __syncthreads();
+    }
+}
+
+// weights_out[t] = decay * weights_in[t] + sum over the head's queries of exp2(s_t - lse).
+__global__ void __launch_bounds__(256) batch_totals_kernel(const DecodeParams p) {
+    pdl_wait();
+    pdl_trigger();
+    const int b = blockIdx.z, h = blockIdx.y;
+    const int n = attended(p.v, p.d, b, false);
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const int G = p.group;
+    const int count = p.base[b + 1] - p.base[b];
+    const float* s = p.scores + (((size_t)p.base[b] * p.v.hkv + (size_t)h * count) * kPageSlots + t) * G;
+    const float* e = p.lse2 + (size_t)b * p.d.n_q_heads + h * G;
+    float sum = 0.f;
+    for (int g = 0; g < G; ++g) sum += exp2_of(s[g] - e[g]);
+    const size_t at = ((size_t)b * p.v.hkv + h) * p.d.weights_stride + t;
+    const bool old = p.d.weights_in && t < p.v.lens[b];
+    p.d.weights_out[at] = old ? p.d.decay * p.d.weights_in[at] + sum : sum;
+}
+
+template <int D>
+constexpr int warps_of() { return D == 256 ? 4 : 8; }
+
+size_t smem_bytes(int batch) { return kRingBytes + sizeof(int) * (size_t)(batch + 1); }
+
+template <typename F>
+cudaError_t for_kernel(bool f16, int dim, bool two, F f) {
+#define GKV_CASE(F16, D, NT) \
+    if (f16 == F16 && dim == D && two == (NT == 2)) return f(batch_decode_kernel<F16, D, NT, warps_of<D>()>);
+    GKV_CASE(false, 64, 1)
+    GKV_CASE(false, 64, 2)
+    GKV_CASE(false, 128, 1)
+    GKV_CASE(false, 128, 2)
+    GKV_CASE(false, 256, 1)
+    GKV_CASE(false, 256, 2)
+    GKV_CASE(true, 64, 1)
+    GKV_CASE(true, 64, 2)
+    GKV_CASE(true, 128, 1)
+    GKV_CASE(true, 128, 2)
+    GKV_CASE(true, 256, 1)
+    GKV_CASE(true, 256, 2)
+#undef GKV_CASE
+    return cudaErrorInvalidValue;
+}
+
+size_t round16(size_t x) { return (x + 15) / 16 * 16; }
+
+struct DecodeSpace {
+    size_t acc, ml, lse2, base, scores, all;
+};
+DecodeSpace decode_space(const BatchView& v, const BatchSplit& s, int n_q_heads, bool totals) {
+    const size_t rows = (size_t)2 * s.workers * s.heads * (n_q_heads / v.hkv);
+    DecodeSpace o;
+    o.acc = 0;
+    o.ml = o.acc + round16(rows * v.dim * sizeof(float));
+    o.lse2 = o.ml + round16(rows * sizeof(float2));
+    o.base = o.lse2 + round16((size_t)v.batch * n_q_heads * sizeof(float));
+    o.scores = o.base + round16((size_t)(v.batch + 1) * sizeof(int32_t));
+    o.all = o.scores + (totals ? (size_t)v.batch * v.table_pages * kPageSlots * n_q_heads * sizeof(float) : 0);
+    return o;
+}
+
+}  // namespace
+
+BatchSplit batch_split(const BatchView& v) {
+    BatchSplit s;
+    s.warps = v.dim == 256 ? 4 : 8;
+    s.heads = v.hkv < s.warps ? v.hkv : s.warps;
+    s.groups = (v.hkv + s.heads - 1) / s.heads;
+    s.lanes = s.warps / s.heads;
+    s.grid = v.sms;
+    s.workers = s.grid * s.lanes;
+    return s;
+}
+
+size_t batch_decode_bytes(const BatchView& v, int32_t n_q_heads, bool totals) {
+    return decode_space(v, batch_split(v), n_q_heads, totals).all;
+}
+
+cudaError_t configure_batch_decode() {
+    for (int f16 = 0; f16 < 2; ++f16)
+        for (int dim = 64; dim <= 256; dim *= 2)
+            for (int two = 0; two < 2; ++two) {
+                cudaError_t e = for_kernel(f16, dim, two, [](auto* k) {
+                    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                (int)smem_bytes(kMaxBatch));
+                });
+                if (e != cudaSuccess) return e;
+            }
+    return cudaSuccess;
+}
+
+cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, cudaStream_t stream) {
+    DecodeParams p;
+    p.v = v;
+    p.d = d;
+    p.s = batch_split(v);
+    p.group = d.n_q_heads / v.hkv;
+    p.min_units = kMinUnits;
+    p.scale_log2 = d.scale * kLog2e;
+    const DecodeSpace o = decode_space(v, p.s, d.n_q_heads, d.weights_out != nullptr);
+    char* w = static_cast<char*>(d.workspace);
+    p.part_acc = reinterpret_cast<float*>(w + o.acc);
+    p.part_ml = reinterpret_cast<float2*>(w + o.ml);
+    p.lse2 = reinterpret_cast<float*>(w + o.lse2);
+    p.base = reinterpret_cast<int32_t*>(w + o.base);
+    p.scores = d.weights_out ? reinterpret_cast<float*>(w + o.scores) : nullptr;
+    cudaError_t e = for_kernel(v.f16, v.dim, p.group > 8, [&](auto* k) {
+        return launch_dependent(k, dim3(p.s.grid), dim3(p.s.warps * 32), smem_bytes(v.batch), stream, p);
+    });
+    if (e != cudaSuccess) return e;
+    // The join is always launched: it also keeps the launches behind it from
+    // starting before the appended rows are in their pages.
+    const int segments = v.batch * p.s.groups;
+    const dim3 grid(segments < 65535 ? segments : 65535, p.s.heads * p.group);
+    e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinWarps * 32), 0, stream, p)
+        : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinWarps * 32), 0, stream, p)
+                       : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinWarps * 32), 0, stream, p);
+    if (e != cudaSuccess || !d.weights_out) return e;
+    return launch_dependent(batch_totals_kernel, dim3((v.table_pages * kPageSlots + 255) / 256, v.hkv, v.batch),
+                            dim3(256), 0, stream, p);
+}
+
+}  // namespace gkv

@@ -476,6 +476,144 @@ int gkv_export_kv(gkv_manager* m, int32_t layer_id, int32_t format, void* K_out,
 int gkv_import_kv(gkv_manager* m, int32_t layer_id, int32_t format, const void* K_in, const void* V_in,
                   const float* k_scales, const float* v_scales, int32_t seq_len, gkv_stream_t stream);
 
+/* ---------------- batches of sequences over one paged pool -----------------
+ * The reference serves one sequence per cache (README.md:150: batch 1). This
+ * tier runs many sequences over ONE K pool and ONE V pool in the same page
+ * layout ([16 slots][Hkv][D]), through a device-resident table and lengths
+ * that the caller owns: nothing here reads a length on the host, so every
+ * call can be captured in a CUDA graph and replayed as the lengths move.
+ *   decode        one new token per sequence: append, attend, and optionally
+ *                 keep a running total of the attention each token received
+ *   page bounds   the smallest and largest key of each page, per dimension
+ *   select pages  the pages whose bound scores highest for a query
+ *   evict         keep the heaviest and the most recent tokens of each head
+ * A sequence with lens[b] < 0 is skipped by every call: nothing of it is
+ * read or written (padding of a fixed-size batch). head_dim 64, 128 or 256;
+ * bf16 or f16; at most 4096 sequences, 256 kv heads, 16 query heads per kv
+ * head. Sequences may share pages for reading; a page that receives a token
+ * (decode) or is compacted (evict) must belong to one sequence alone.
+ * Every pointer is device memory on `device`; calls allocate nothing and
+ * synchronise nothing. Scratch is the caller's `workspace` (16-byte aligned;
+ * calls that may overlap on the GPU need one each). */
+typedef struct gkv_batch {
+    gkv_pool_desc pool;
+    const int32_t* table;  /* [batch][table_stride][2] {k_id, v_id} */
+    const int32_t* lens;   /* [batch] cached tokens of each sequence, < 0: skipped */
+    int64_t table_stride;  /* entries from one row to the next, >= table_pages */
+    int32_t batch;
+    int32_t table_pages;   /* entries of each row; tokens behind them are not reached */
+    int32_t device;
+} gkv_batch;
+
+/* Look up what later calls on `device` need (error word, kernel
+ * attributes). Calls do this themselves when it has not been done; call it
+ * before a stream capture that holds the first of them. */
+int gkv_batch_prepare(int device);
+
+/* Synchronise `device`, read and clear its batch error word (GKV_ERR_DEVICE
+ * when set): bit 0 = a page id outside the pool, that page was skipped;
+ * bit 2 = a length beyond the table row, the tokens behind it were left out. */
+int gkv_batch_check_errors(int device, uint32_t* flags);
+
+typedef struct gkv_batch_decode_args {
+    const void* q;           /* [batch][Hq][D], rows 16-byte aligned, strides in elements */
+    int64_t q_stride_batch, q_stride_head;
+    const void* k_new;       /* [batch][Hkv][D] this step's token, or both NULL: attend only */
+    const void* v_new;
+    int64_t k_stride_batch, k_stride_head, v_stride_batch, v_stride_head;
+    void* out;               /* [batch][Hq][D] contiguous */
+    float* lse;              /* [batch][Hq] natural log of the sum of exponentials, or NULL */
+    const int32_t* pages;    /* [batch][Hkv][n_pages] logical pages to attend, or NULL: all */
+    const float* weights_in; /* [batch][Hkv][weights_stride], or NULL: zeros */
+    float* weights_out;      /* the same shape, may be weights_in; NULL: no totals */
+    int64_t weights_stride;  /* >= 16 * table_pages */
+    int32_t n_pages;
+    int32_t n_q_heads;
+    int32_t out_dtype;
+    float scale;
+    float decay;
+    void* workspace;
+    size_t workspace_bytes;
+} gkv_batch_decode_args;
+
+/* Bytes of workspace gkv_batch_decode needs with n_q_heads query heads, with
+ * (totals != 0) or without weights_out. */
+int gkv_batch_decode_workspace(const gkv_batch* b, int32_t n_q_heads, int32_t totals, size_t* bytes);
+
+/* One decode step. With k_new / v_new the token is written at position
+ * lens[b] (its page must be in the table) and attended with the lens[b]
+ * cached ones; lens itself stays as it is: the caller adds 1 before the next
+ * step. A sequence with no token to attend gets zeros and lse -inf.
+ * With `pages`, KV head h of sequence b attends only the listed logical
+ * pages: the first min(n_pages, pages in use) entries of its list are read,
+ * entries outside the pages in use (such as -1) are skipped, a page listed
+ * twice counts twice; the new token is appended in any case and attended when
+ * its page is listed. With weights_out (not together with `pages`):
+ *   weights_out[b][h][t] = decay * weights_in[b][h][t] + sum over the query
+ *   heads of h of the attention weight of token t
+ * for every attended t; the new token's weights_in counts as 0. */
+int gkv_batch_decode(const gkv_batch* b, const gkv_batch_decode_args* a, gkv_stream_t stream);
+
+/* bounds [pool_pages][Hkv][2][D] in the pool's dtype, indexed by K page id:
+ * for every page of a sequence holding one of the tokens [start[b], lens[b] +
+ * extra) (start NULL: 0), the smallest (0) and the largest (1) value of each
+ * key dimension over the page's tokens below lens[b] + extra. NaN spreads. */
+int gkv_batch_page_bounds(const gkv_batch* b, const int32_t* start, int32_t extra, void* bounds,
+                          gkv_stream_t stream);
+
+typedef struct gkv_batch_select_args {
+    const void* q;        /* as in gkv_batch_decode_args */
+    int64_t q_stride_batch, q_stride_head;
+    const void* bounds;   /* of gkv_batch_page_bounds */
+    int32_t* pages;       /* [batch][Hkv][n_pages] */
+    int32_t n_pages;
+    int32_t n_first;      /* pages at the start that are always taken */
+    int32_t n_last;       /* pages at the end that are always taken */
+    int32_t extra;        /* tokens the sequence is about to gain (1 before a decode step that appends) */
+    int32_t n_q_heads;
+    void* workspace;
+    size_t workspace_bytes;
+} gkv_batch_select_args;
+
+int gkv_batch_select_workspace(const gkv_batch* b, size_t* bytes);
+
+/* For each sequence and KV head, the n_pages logical pages with the largest
+ *   max over the query heads g of h of  sum_d (q_gd >= 0 ? q_gd * max_d : q_gd * min_d),
+ * an upper bound of the page's scores, computed in 64 bits; equal ones go to
+ * the lower page, a NaN bound is taken first. The first n_first and last
+ * n_last pages are taken whatever their bounds, which are not used (n_first +
+ * n_last <= n_pages). Written in rising order, -1 behind the last one. */
+int gkv_batch_select_pages(const gkv_batch* b, const gkv_batch_select_args* a, gkv_stream_t stream);
+
+typedef struct gkv_batch_evict_args {
+    const float* weights;      /* [batch][Hkv][stride] */
+    float* weights_out;        /* the same shape, may be `weights` */
+    const int32_t* positions;  /* [batch][Hkv][stride], used below tracked[b]; NULL only with tracked NULL */
+    int32_t* positions_out;    /* the same shape, may be `positions` */
+    const int32_t* seen;       /* [batch] tokens the sequence has had in all: the next token's position */
+    const int32_t* tracked;    /* [batch] slots whose position is in `positions`, or NULL: none */
+    int32_t* lens_out;         /* [batch], may be lens */
+    int64_t stride;            /* >= 16 * table_pages */
+    int32_t n_keep;
+    int32_t n_recent;          /* <= n_keep */
+    void* workspace;
+    size_t workspace_bytes;
+} gkv_batch_evict_args;
+
+int gkv_batch_evict_workspace(const gkv_batch* b, size_t* bytes);
+
+/* Cut every sequence back to at most n_keep tokens, each KV head keeping its
+ * own: first the tokens at positions >= seen[b] - n_recent, then those with
+ * the largest weights (NaN first; equal ones by the lower slot). Slot t holds
+ * position positions[b][h][t] below tracked[b], seen[b] - (lens[b] - t) from
+ * there on (appended since). Kept rows below the new length left = min(lens,
+ * n_keep) stay; the i-th slot that became free there takes K, V, weight and
+ * position of the i-th kept slot behind it. weights_out and positions_out are
+ * written for all slots below left, lens_out[b] = left: pass that as `tracked`
+ * next time. Keys carry their rotation, so attention does not mind the order.
+ * Pages behind the new length are the caller's to free. */
+int gkv_batch_evict(const gkv_batch* b, const gkv_batch_evict_args* a, gkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

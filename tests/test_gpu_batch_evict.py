@@ -1,0 +1,201 @@
+"""gkv_batch_evict against its definition, and runs of the batch operators together."""
+import math
+
+import pytest
+import torch
+
+import batch_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+LENS = [0, 1, 40, 64, -1, 300, 1500]
+
+
+def cache_of(c):
+    from genllm_b200.batch import PagedBatch
+    return PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+
+
+def same(a, b):
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+def check(c, w, seen, keep, recent, tracked=None, positions=None, in_place=False):
+    from genllm_b200.batch import CacheEvict
+    want = ref.evict(c, w, seen, keep, recent, tracked, positions)
+    cache = cache_of(c)
+    if in_place:
+        options = dict(lens_out=c.lens)
+    else:
+        first_positions = positions if positions is not None else torch.zeros(w.shape, dtype=torch.int32, device="cuda")
+        options = dict(weights_out=w.clone(), positions_out=first_positions.clone(), lens_out=c.lens.clone())
+    old = w.clone()
+    op = CacheEvict(cache, w, seen, keep=keep, recent=recent, tracked=tracked, positions=positions, **options)
+    lens = op.run()
+    assert cache.check_device_errors() == 0
+    assert torch.equal(lens, want[0])
+    assert torch.equal(op.weights_out.view(torch.int32), want[1].view(torch.int32))
+    assert torch.equal(op.positions_out, want[2])
+    assert same(c.k_pool, want[3]) and same(c.v_pool, want[4])
+    if not in_place:
+        assert torch.equal(w.view(torch.int32), old.view(torch.int32))
+    return op
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("keep,recent", [(0, 0), (1, 0), (1, 1), (17, 5), (64, 64), (128, 0), (1499, 30), (5000, 10)])
+@pytest.mark.parametrize("hkv,d,dtype", [(2, 64, torch.float16), (3, 128, torch.bfloat16), (1, 256, torch.bfloat16)])
+def test_first_eviction(hkv, d, dtype, keep, recent, in_place):
+    c = ref.make_case(LENS, hkv, hkv, d, dtype, seed=keep)
+    g = torch.Generator("cuda").manual_seed(keep)
+    w = torch.rand((len(LENS), hkv, 16 * c.table.shape[1]), generator=g, device="cuda") ** 4
+    check(c, w, c.lens.clamp(min=0) + 3, keep, recent, in_place=in_place)
+
+
+def test_tracked_positions():
+    """Slots kept before hold tokens of any age; those appended since are in order."""
+    lens = [100, 333, 50]
+    c = ref.make_case(lens, 2, 2, 64, torch.bfloat16, seed=1)
+    g = torch.Generator().manual_seed(2)
+    width = 16 * c.table.shape[1] + 5
+    tracked, seen = torch.tensor([64, 300, 50], dtype=torch.int32), torch.tensor([500, 1000, 60], dtype=torch.int32)
+    positions = torch.zeros(3, 2, width, dtype=torch.int32)
+    for b in range(3):
+        for h in range(2):
+            old = int(seen[b]) - (lens[b] - int(tracked[b]))
+            positions[b, h, :tracked[b]] = torch.randperm(old, generator=g)[:tracked[b]].int()
+    w = torch.rand(3, 2, width, generator=g).cuda()
+    check(c, w, seen.cuda(), 40, 25, tracked.cuda(), positions.cuda())
+
+
+def test_equal_weights_infinities_and_nan():
+    c = ref.make_case([200], 4, 4, 64, torch.float16, seed=3)
+    w = torch.zeros(1, 4, 16 * c.table.shape[1], device="cuda")
+    w[0, 1, ::2] = -0.0
+    w[0, 2] = torch.randint(0, 3, w[0, 2].shape, device="cuda").float()
+    w[0, 3, :200] = torch.randn(200, device="cuda")
+    w[0, 3, 100], w[0, 3, 150], w[0, 3, 151], w[0, 3, 10] = math.nan, math.inf, -math.inf, -math.nan
+    check(c, w, c.lens.clone(), 30, 7)
+    c = ref.make_case([200], 4, 4, 64, torch.float16, seed=3)
+    check(c, w, c.lens.clone(), 1, 0)
+
+
+def test_long_rows_and_repeats():
+    c = ref.make_case([20000, 9000], 2, 2, 64, torch.bfloat16, seed=4)
+    w = torch.rand((2, 2, 16 * c.table.shape[1]), device="cuda")
+    check(c, w, c.lens.clone(), 8192, 100)
+
+
+def test_bad_pages_are_flagged():
+    from genllm_b200.batch import CacheEvict
+    c = ref.make_case([100], 2, 2, 64, torch.bfloat16, seed=5)
+    w = torch.rand((1, 2, 16 * c.table.shape[1]), device="cuda")
+    cache = cache_of(c)
+    c.table[0, 5, 1] = 1 << 20
+    CacheEvict(cache, w, c.lens.clone(), keep=20).run()
+    assert cache.check_device_errors() == 1
+    c.lens[0] = 1 << 30
+    c.table[0, 5, 1] = 0
+    CacheEvict(cache, w, c.lens.clone(), keep=20).run()
+    assert cache.check_device_errors() & 4
+
+
+def test_captured_eviction():
+    from genllm_b200.batch import CacheEvict
+    c = ref.make_case([500, 90], 2, 2, 64, torch.bfloat16, seed=6)
+    w = torch.rand((2, 2, 16 * c.table.shape[1]), device="cuda")
+    seen = c.lens.clone()
+    want = ref.evict(c, w, seen, 70, 8)
+    op = CacheEvict(cache_of(c), w, seen, keep=70, recent=8, lens_out=c.lens)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op.run()
+    graph.replay()
+    assert torch.equal(c.lens, want[0]) and same(c.k_pool, want[3]) and same(c.v_pool, want[4])
+    assert torch.equal(w, want[1])
+
+
+def test_decode_with_totals_then_eviction_over_many_steps():
+    """A serving loop on a budget: append and attend, total the attention, cut
+    back every 16 steps; the cache holds the tokens an ideal one would."""
+    from genllm_b200.batch import BatchDecode, CacheEvict, PagedBatch
+    hq, hkv, d, keep, recent = 8, 2, 64, 48, 12
+    lens = [0, 30, 60]
+    c = ref.make_case(lens, hq, hkv, d, torch.bfloat16, seed=9, width=5, spare=1)
+    batch, width = 3, 5 * 16
+    # Room for keep + 16 tokens in every row.
+    total = batch * 5
+    pools = [torch.zeros(total, 16, hkv, d, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    g = torch.Generator("cuda").manual_seed(10)
+    table = torch.stack([torch.randperm(total, generator=g, device="cuda").view(batch, 5) for _ in range(2)], -1).int()
+    for b, n in enumerate(lens):
+        for t in range(n):
+            for w, (mine, theirs) in enumerate(((pools[0], c.k_pool), (pools[1], c.v_pool))):
+                mine[int(table[b, t // 16, w]), t % 16] = theirs[int(c.table[b, t // 16, w]), t % 16]
+    c.k_pool, c.v_pool, c.table = pools[0], pools[1], table
+    cache = PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+    weights = torch.zeros(batch, hkv, width, device="cuda")
+    positions = torch.zeros(batch, hkv, width, dtype=torch.int32, device="cuda")
+    tracked, seen = torch.zeros(batch, dtype=torch.int32, device="cuda"), c.lens.clone()
+    step = BatchDecode(cache, c.q, c.k_new, c.v_new, weights=weights, weights_out=weights, decay=0.95)
+    cut = CacheEvict(cache, weights, seen, keep=keep, recent=recent, tracked=tracked, positions=positions, lens_out=c.lens)
+    for i in range(40):
+        for t in (c.q, c.k_new, c.v_new):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda").to(t.dtype))
+        want = ref.decode(c)
+        step.run()
+        ref.check_close(step.out, want["out"], want["slack"], f"step {i}")
+        c.lens += 1
+        seen += 1
+        if i % 16 == 15:
+            expect = ref.evict(c, weights, seen, keep, recent, tracked, positions)
+            cut.run()
+            tracked.copy_(c.lens)
+            assert torch.equal(c.lens, expect[0]) and torch.equal(weights, expect[1]) and torch.equal(positions, expect[2])
+            assert same(c.k_pool, expect[3]) and same(c.v_pool, expect[4])
+            for b in range(batch):
+                kept = positions[b, :, :int(c.lens[b])]
+                for h in range(hkv):  # the most recent tokens are all there
+                    assert set(range(max(0, int(seen[b]) - recent), int(seen[b]))) <= set(kept[h].tolist())
+    assert cache.check_device_errors() == 0
+
+
+def test_managed_prompt_then_sparse_steps():
+    """A prompt through the manager's chunk path, then sparse and dense steps over the layer's own pages."""
+    from genllm_b200.batch import BatchDecode, PageBounds, PagedBatch, PageSelect
+    from genllm_b200.paged_attention import PagedAttentionManager, paged_attention
+    g = torch.Generator("cuda").manual_seed(3)
+    hq, hkv, d, prompt = 16, 8, 128, 300
+    randn = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    m = PagedAttentionManager(0)
+    m.init_layer(0, hkv, d)
+    m.reserve_layer(0, 40)
+    paged_attention(m, 0, randn(1, hq, prompt, d), randn(1, hkv, prompt, d), randn(1, hkv, prompt, d))
+    m.append_kv_pages(0, 40)  # room for the steps to come
+    k_ids, v_ids = m.page_table(0)
+    k_pool, v_pool = m.pool_tensors(0)
+    table = torch.tensor([list(zip(k_ids, v_ids))], dtype=torch.int32, device="cuda")
+    c = ref.Case(k_pool, v_pool, table, torch.tensor([prompt], dtype=torch.int32, device="cuda"), randn(1, hq, d),
+                 randn(1, hkv, d), randn(1, hkv, d))
+    cache = PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+    bound = PageBounds(cache, torch.zeros(40, hkv, 2, d, dtype=torch.bfloat16, device="cuda")).run()
+    select = PageSelect(cache, c.q, bound, 6, first=1, last=2)
+    step = BatchDecode(cache, c.q, c.k_new, c.v_new, pages=select.pages)
+    refresh = PageBounds(cache, bound, start=c.lens, extra=1)
+    for _ in range(20):
+        for t in (c.q, c.k_new, c.v_new):
+            t.copy_(randn(*t.shape))
+        pages = ref.select(c, bound, 6, 1, 2, 1)
+        want = ref.decode(c, pages=pages)
+        want_bounds = bound.clone()
+        select.run()
+        step.run()
+        refresh.run()
+        assert torch.equal(select.pages.cpu(), pages)
+        ref.check_close(step.out, want["out"], want["slack"])
+        assert same(bound, ref.bounds(c, want_bounds, start=c.lens, extra=1))
+        c.lens += 1
+    want = ref.decode(c)
+    dense = BatchDecode(cache, c.q, c.k_new, c.v_new)
+    ref.check_close(dense.run(), want["out"], want["slack"])
+    assert cache.check_device_errors() == 0
