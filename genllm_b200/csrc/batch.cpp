@@ -90,7 +90,7 @@ int check_batch(const gkv_batch* b) {
     if (p.head_dim != 64 && p.head_dim != 128 && p.head_dim != 256)
         return fail(GKV_ERR_UNSUPPORTED, "head_dim %d: 64, 128 and 256 are built", p.head_dim);
     if (p.n_kv_heads < 1 || p.n_kv_heads > kMaxKvHeads) return fail(GKV_ERR_INVALID, "n_kv_heads %d", p.n_kv_heads);
-    if (p.pool_pages < 1) return fail(GKV_ERR_INVALID, "pool_pages %d", p.pool_pages);
+    if (p.pool_pages < 1 || p.pool_pages > INT32_MAX / GKV_PAGE_SLOTS) return fail(GKV_ERR_INVALID, "pool_pages %d", p.pool_pages);
     if (!p.k_base || !p.v_base || !aligned(p.k_base, 16) || !aligned(p.v_base, 16))
         return fail(GKV_ERR_INVALID, "pool bases must be non-null and 16-byte aligned");
     if (b->batch < 1 || b->batch > gkv::kMaxBatch)

@@ -5,22 +5,38 @@
 // they are; the i-th slot that became free there takes the i-th kept slot at
 // or behind `left`. Sources lie at or behind `left`, destinations before it,
 // so the rows move in place, in any order, and the fewest rows move.
+//
+// The plan kernel reads each weight once into shared memory as an ordered
+// integer and cuts the row there (cut.cuh); the move kernel is a copy, bound
+// by HBM: 4 row lengths per move (K and V, read and written).
 #include <algorithm>
 
 #include "batch.cuh"
+#include "cut.cuh"
 
 namespace gkv {
 namespace {
 
+// One kept row behind the new length and the slot it goes to.
+struct __align__(16) Move {
+    int to, from;
+    float weight;
+    int position;
+};
+
 struct EvictParams {
     BatchView v;
     EvictLaunch e;
-    int32_t* counts;  // [batch * hkv] moves of each head
-    int32_t* left;    // [batch] new length, -1: skipped
-    int2* moves;      // [batch * hkv][16 * table_pages] {to, from}
+    int32_t* counts;   // [batch * hkv] moves of each head
+    int32_t* left;     // [batch] new length, -1: skipped
+    Move* moves;       // [batch * hkv][16 * table_pages]
+    uint32_t* keys;    // [batch * hkv][16 * table_pages] where a slice does not fit in shared memory; else null
 };
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kBatch = 8;          // loads of a thread in flight
+constexpr int kMaxSlice = 40960;  // keys of a CTA in shared memory: 160 KB
 constexpr uint32_t kRecent = ~0u, kNaN32 = ~0u - 1;
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -29,156 +45,240 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// The positions of the CTA's threads that hold `flag`, in thread order: how
-// many before this one; *all how many in all. sums: one int per warp.
-__device__ __forceinline__ int rank_of(bool flag, int* sums, int* all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t mask = __ballot_sync(0xFFFFFFFFu, flag);
-    __syncthreads();
-    if (lane == 0) sums[warp] = __popc(mask);
-    __syncthreads();
-    int before = __popc(mask & ((1u << lane) - 1)), total = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
-    }
-    *all = total;
-    return before;
-}
-
-__global__ void __launch_bounds__(kPlanThreads) evict_plan_kernel(const EvictParams p) {
-    __shared__ int hist[256];
-    __shared__ int found[2];
-    __shared__ int sums[kPlanThreads / 32];
+// One cluster per (sequence, head), one slice of its slots per CTA; a warp
+// takes a run of its slice, so ranks in slot order are ballots and prefix sums.
+__global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const EvictParams p) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint32_t slice_keys[];
+    __shared__ CutShared<uint32_t, kPlanThreads> cut_shared;
+    __shared__ int slots[kPlanWarps];
+    __shared__ int2 rank_slots[2][kMaxCluster];
     pdl_trigger();
     pdl_wait();
+    cg::cluster_group cluster = cg::this_cluster();
     const BatchView& v = p.v;
-    const int tid = threadIdx.x, bh = blockIdx.x, b = bh / v.hkv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int bh = blockIdx.x / ranks, b = bh / v.hkv;
     const int len = v.lens[b];
     const int cap = v.table_pages * kPageSlots;
-    if (len > cap && tid == 0) atomicOr(v.err, kErrBadLength);
+    const bool first = rank == 0 && tid == 0;
+    if (len > cap && first) atomicOr(v.err, kErrBadLength);
     const int n = min(len, cap), left = min(n, p.e.n_keep);
-    if (tid == 0) {
+    if (first) {
         if (bh % v.hkv == 0) p.left[b] = len < 0 ? -1 : left;
-        if (n <= left) p.counts[bh] = 0;
+        if (n <= left || left == 0) p.counts[bh] = 0;
     }
-    if (len < 0) return;
+    if (len < 0 || left == 0) return;  // the whole cluster
     const size_t row = (size_t)bh * p.e.stride;
     const float* weights = p.e.weights + row;
     const int seen = p.e.seen[b], tracked = p.e.tracked ? p.e.tracked[b] : 0;
     auto position = [&](int t) { return t < tracked ? p.e.positions[row + t] : seen - (n - t); };
+    const bool same_weights = p.e.weights_out == p.e.weights;
+    const bool same_positions = p.e.positions_out == p.e.positions;
+    // What a slot that stays keeps; in place there is little to write.
+    auto stay = [&](int t, float w, int pos) {
+        if (!same_weights) p.e.weights_out[row + t] = w;
+        if (!same_positions || t >= tracked) p.e.positions_out[row + t] = pos;
+    };
     if (n <= left) {
-        for (int t = tid; t < n; t += kPlanThreads) {
-            p.e.weights_out[row + t] = weights[t];
-            p.e.positions_out[row + t] = position(t);
-        }
-        return;
+        for (int t = rank * kPlanThreads + tid; t < n; t += ranks * kPlanThreads) stay(t, weights[t], position(t));
+        return;  // the whole cluster
     }
-    auto key = [&](int t) { return position(t) >= seen - p.e.n_recent ? kRecent : key_of(weights[t]); };
-    // The smallest kept key, byte by byte from the top.
-    uint32_t prefix = 0;
-    int want = left;
-    for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kPlanThreads) hist[i] = 0;
-        __syncthreads();
-        for (int t = tid; t < n; t += kPlanThreads) {
-            const uint32_t k = key(t);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+    // This CTA's slots [s0, s0 + m).
+    const int slice = ((n + ranks - 1) / ranks + 31) / 32 * 32;
+    const int s0 = min(n, rank * slice), m = min(n - s0, slice);
+    uint32_t* keys = p.keys ? p.keys + (size_t)bh * cap + s0 : slice_keys;
+    for (int i = tid; i < m; i += kBatch * kPlanThreads) {
+        // All loads of a batch first: the row comes from HBM.
+        float w[kBatch];
+        int at[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int t = s0 + min(i + j * kPlanThreads, m - 1);
+            w[j] = weights[t];
+            at[j] = position(t);
         }
-        __syncthreads();
-        if (tid == 0) {
-            int rest = want, d = 255;
-            while (d > 0 && hist[d] < rest) rest -= hist[d--];
-            found[0] = d;
-            found[1] = rest;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)found[0] << shift;
-        want = found[1];
-        __syncthreads();
-    }
-    // In slot order: `want` of the slots with that key stay, and all above it.
-    int2* moves = p.moves + (size_t)bh * v.table_pages * kPageSlots;
-    int equal = 0, holes = 0, sources = 0;
-    for (int t0 = 0; t0 < n; t0 += kPlanThreads) {
-        const int t = t0 + tid;
-        const uint32_t k = t < n ? key(t) : 0;
-        int all;
-        const int same_before = equal + rank_of(t < n && k == prefix, sums, &all);
-        equal += all;
-        const bool kept = t < n && left > 0 && (k > prefix || (k == prefix && same_before < want));
-        const bool hole = t < left && !kept, source = kept && t >= left;
-        const int hole_at = holes + rank_of(hole, sums, &all);
-        holes += all;
-        const int source_at = sources + rank_of(source, sums, &all);
-        sources += all;
-        if (hole) moves[hole_at].x = t;
-        if (source) moves[source_at].y = t;
-        if (t < left && kept) {
-            const int pos = position(t);
-            const float w = weights[t];
-            p.e.weights_out[row + t] = w;
-            p.e.positions_out[row + t] = pos;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (i + j * kPlanThreads >= m) break;
+            const bool is_recent = at[j] >= seen - p.e.n_recent;
+            keys[i + j * kPlanThreads] = is_recent ? kRecent : key_of(w[j]);
         }
     }
     __syncthreads();
-    for (int i = tid; i < holes; i += kPlanThreads) {
-        const int2 m = moves[i];
-        p.e.weights_out[row + m.x] = weights[m.y];
-        p.e.positions_out[row + m.x] = position(m.y);
+    uint32_t top = 0;
+    const Cut<uint32_t> cut = cluster_cut<uint32_t, kPlanThreads>(keys, m, left, kRecent, &top, cut_shared);
+
+    // A warp's run of the slice.
+    const int run = ((m + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+    const int i0 = min(m, warp * run), i1 = min(m, i0 + run);
+    const uint32_t below = (1u << lane) - 1;
+    int equal = 0;  // keys of the cut's range before this run, in slot order
+    if (cut.partial) {
+        int mine = 0;
+        for (int i = i0 + lane; i < i1; i += 32) mine += keys[i] >= cut.lo && keys[i] <= cut.hi;
+        mine = __reduce_add_sync(~0u, mine);
+        int all;
+        equal = warps_before<kPlanThreads>(mine, slots, &all);
+        equal += cluster_before(make_int2(all, 0), rank_slots[0]).x;
     }
-    if (tid == 0) p.counts[bh] = holes;
+    auto kept_of = [&](int i, int* seen_equal) {
+        const uint32_t k = i < i1 ? keys[i] : 0;
+        const bool in = i < i1 && k >= cut.lo && k <= cut.hi;
+        bool kept = i < i1 && (k > cut.hi || in);
+        if (cut.partial) {
+            const uint32_t mask = __ballot_sync(~0u, in);
+            if (in) kept = *seen_equal + __popc(mask & below) < cut.ties;
+            *seen_equal += __popc(mask);
+        }
+        return kept;
+    };
+    int holes = 0, sources = 0, at = equal;
+    for (int i = i0; i < i1; i += 32) {
+        const bool kept = kept_of(i + lane, &at);
+        const int t = s0 + i + lane;
+        holes += __popc(__ballot_sync(~0u, i + lane < i1 && t < left && !kept));
+        sources += __popc(__ballot_sync(~0u, kept && t >= left));
+    }
+    int hole_all, source_all;
+    int hole_at = warps_before<kPlanThreads>(holes, slots, &hole_all);
+    int source_at = warps_before<kPlanThreads>(sources, slots, &source_all);
+    const int2 before = cluster_before(make_int2(hole_all, source_all), rank_slots[1]);
+    hole_at += before.x;
+    source_at += before.y;
+    if (rank == ranks - 1 && tid == kPlanThreads - 1) {
+        // The last run's end: the count of the whole row.
+        p.counts[bh] = hole_at + holes;
+    }
+    Move* moves = p.moves + (size_t)bh * cap;
+    at = equal;
+    for (int ib = i0; ib < i1; ib += 32 * kBatch) {
+        float w[kBatch];
+        int pos[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int t = s0 + min(ib + j * 32 + lane, m - 1);
+            w[j] = weights[t];
+            pos[j] = position(t);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = ib + j * 32;
+            if (i >= i1) break;
+            const bool kept = kept_of(i + lane, &at);
+            const int t = s0 + i + lane;
+            const bool hole = i + lane < i1 && t < left && !kept, source = kept && t >= left;
+            const uint32_t hole_mask = __ballot_sync(~0u, hole), source_mask = __ballot_sync(~0u, source);
+            if (hole) moves[hole_at + __popc(hole_mask & below)].to = t;
+            if (source) {
+                Move& mv = moves[source_at + __popc(source_mask & below)];
+                mv.from = t;
+                mv.weight = w[j];
+                mv.position = pos[j];
+            }
+            if (kept && t < left) stay(t, w[j], pos[j]);
+            hole_at += __popc(hole_mask);
+            source_at += __popc(source_mask);
+        }
+    }
 }
 
 constexpr int kMoveThreads = 256;
 
-// Moves the rows: one warp per move, K and V.
+// Moves the rows, kGroup moves of a warp in flight: lane j holds the K rows of
+// move j, lane kGroup + j its V rows; then all lanes copy, 16 bytes each.
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
-    constexpr int kChunks = D / 8;
+    constexpr int kChunks = D / 8, kGroup = D == 256 ? 4 : 8;
+    constexpr int kCopies = kGroup * 2 * kChunks / 32;  // of a lane
     pdl_wait();
     const BatchView& v = p.v;
     const int lane = threadIdx.x & 31;
     const int bh = blockIdx.y, b = bh / v.hkv, h = bh % v.hkv;
-    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0 && p.left[b] >= 0) p.e.lens_out[b] = p.left[b];
-    if (p.left[b] < 0) return;
-    const int count = p.counts[bh];
-    const int2* moves = p.moves + (size_t)bh * v.table_pages * kPageSlots;
+    const int left = p.left[b], count = p.counts[bh];
+    if (left < 0) return;
+    if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) p.e.lens_out[b] = left;
+    const Move* moves = p.moves + (size_t)bh * v.table_pages * kPageSlots;
     const int2* table = v.table + b * v.table_stride;
-    for (int i = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); i < count; i += gridDim.x * (kMoveThreads / 32)) {
-        const int2 m = moves[i];
-        const int2 to = table[m.x / kPageSlots], from = table[m.y / kPageSlots];
-        if (min(min(to.x, to.y), min(from.x, from.y)) < 0 || max(max(to.x, to.y), max(from.x, from.y)) >= v.pool_pages) {
-            if (lane == 0) atomicOr(v.err, kErrBadPage);
-            continue;
+    const int step = gridDim.x * (kMoveThreads / 32) * kGroup;
+    for (int i0 = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kGroup; i0 < count; i0 += step) {
+        const int mine = lane % kGroup;
+        int to_row = -1, from_row = -1;
+        if (lane < 2 * kGroup && i0 + mine < count) {
+            const Move m = moves[i0 + mine];
+            const int2 to = table[m.to / kPageSlots], from = table[m.from / kPageSlots];
+            if (lane < kGroup) {
+                p.e.weights_out[(size_t)bh * p.e.stride + m.to] = m.weight;
+                p.e.positions_out[(size_t)bh * p.e.stride + m.to] = m.position;
+            }
+            if (min(min(to.x, to.y), min(from.x, from.y)) < 0 ||
+                max(max(to.x, to.y), max(from.x, from.y)) >= v.pool_pages) {
+                atomicOr(v.err, kErrBadPage);
+            } else {
+                to_row = (lane < kGroup ? to.x : to.y) * kPageSlots + m.to % kPageSlots;
+                from_row = (lane < kGroup ? from.x : from.y) * kPageSlots + m.from % kPageSlots;
+            }
         }
-        for (int c = lane; c < 2 * kChunks; c += 32) {
+        uint4 x[kCopies];
+        uint4* dst[kCopies];
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) {
+            const int at = k * 32 + lane, c = at % (2 * kChunks);
             const bool is_v = c >= kChunks;
-            uint16_t* pool = is_v ? v.v_base : v.k_base;
-            const size_t src = ((size_t)(is_v ? from.y : from.x) * kPageSlots + m.y % kPageSlots) * v.hkv + h;
-            const size_t dst = ((size_t)(is_v ? to.y : to.x) * kPageSlots + m.x % kPageSlots) * v.hkv + h;
-            reinterpret_cast<uint4*>(pool + dst * D)[c % kChunks] = reinterpret_cast<const uint4*>(pool + src * D)[c % kChunks];
+            const int holder = at / (2 * kChunks) + (is_v ? kGroup : 0);
+            const int from = __shfl_sync(~0u, from_row, holder), to = __shfl_sync(~0u, to_row, holder);
+            uint4* pool = reinterpret_cast<uint4*>(is_v ? v.v_base : v.k_base);
+            dst[k] = to < 0 ? nullptr : pool + ((size_t)to * v.hkv + h) * kChunks + c % kChunks;
+            if (to >= 0) x[k] = pool[((size_t)from * v.hkv + h) * kChunks + c % kChunks];
         }
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k)
+            if (dst[k]) *dst[k] = x[k];
     }
 }
 
 size_t round16(size_t x) { return (x + 15) / 16 * 16; }
 
-}  // namespace
-
-size_t evict_bytes(const BatchView& v) {
-    const size_t heads = (size_t)v.batch * v.hkv;
-    return round16(heads * 4) + round16((size_t)v.batch * 4) + heads * v.table_pages * kPageSlots * sizeof(int2);
+struct EvictSpace {
+    int cluster;
+    bool spill;  // keys in the workspace
+    size_t left, moves, keys, all;
+};
+EvictSpace evict_space(const BatchView& v) {
+    const size_t heads = (size_t)v.batch * v.hkv, cap = (size_t)v.table_pages * kPageSlots;
+    EvictSpace s;
+    s.cluster = cluster_for((int)heads, (int64_t)cap, v.sms, 2048, kMaxSlice);
+    s.spill = (cap + s.cluster - 1) / s.cluster > kMaxSlice;
+    s.left = round16(heads * sizeof(int32_t));
+    s.moves = s.left + round16((size_t)v.batch * sizeof(int32_t));
+    s.keys = s.moves + heads * cap * sizeof(Move);
+    s.all = s.keys + (s.spill ? heads * cap * sizeof(uint32_t) : 0);
+    return s;
 }
 
-cudaError_t configure_evict() { return cudaSuccess; }
+}  // namespace
+
+size_t evict_bytes(const BatchView& v) { return evict_space(v).all; }
+
+cudaError_t configure_evict() {
+    return cudaFuncSetAttribute(evict_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kMaxSlice * (int)sizeof(uint32_t));
+}
 
 cudaError_t launch_evict(const BatchView& v, const EvictLaunch& e, cudaStream_t stream) {
-    const size_t heads = (size_t)v.batch * v.hkv;
+    const size_t heads = (size_t)v.batch * v.hkv, cap = (size_t)v.table_pages * kPageSlots;
+    const EvictSpace s = evict_space(v);
     char* w = static_cast<char*>(e.workspace);
-    EvictParams p{v, e, reinterpret_cast<int32_t*>(w), reinterpret_cast<int32_t*>(w + round16(heads * 4)),
-                  reinterpret_cast<int2*>(w + round16(heads * 4) + round16((size_t)v.batch * 4))};
-    cudaError_t err = launch_dependent(evict_plan_kernel, dim3((unsigned)heads), dim3(kPlanThreads), 0, stream, p);
+    EvictParams p{v,
+                  e,
+                  reinterpret_cast<int32_t*>(w),
+                  reinterpret_cast<int32_t*>(w + s.left),
+                  reinterpret_cast<Move*>(w + s.moves),
+                  s.spill ? reinterpret_cast<uint32_t*>(w + s.keys) : nullptr};
+    const size_t slice = ((cap + s.cluster - 1) / s.cluster + 31) / 32 * 32;
+    cudaError_t err = launch_cluster(evict_plan_kernel, (unsigned)heads, s.cluster, kPlanThreads,
+                                     s.spill ? 0 : slice * sizeof(uint32_t), stream, p);
     if (err != cudaSuccess) return err;
     // About eight CTAs per SM over all heads.
     const int x = (int)std::max<size_t>(1, (size_t)v.sms * 8 / heads);
