@@ -19,6 +19,8 @@
 // per-warp cp.async ring, 16-byte chunks XOR-permuted by row for ldmatrix.
 // mma.sync and not tcgen05: at 16 query heads or fewer the products are far
 // below the stream of K and V in cost, and each warp works without barriers.
+#include <algorithm>
+
 #include "batch.cuh"
 
 namespace gkv {
@@ -27,15 +29,15 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kMinUnits = 4;  // pages of a worker at least: below that the join costs more than it spreads
+constexpr int kMaxGrid = 160;  // bounds the parts of a sequence: kMaxGrid workers times 8 to a CTA
 constexpr int kRingBytes = 192 * 1024;
+constexpr int kRingAlign = 512;  // the longest row: chunk offsets in a row are XORs of its address
 
 struct DecodeParams {
     BatchView v;
     BatchDecodeLaunch d;
     BatchSplit s;
     int32_t group;       // query heads per kv head
-    int32_t min_units;
     float scale_log2;
     float* part_acc;     // [2 workers][heads * group][D]
     float2* part_ml;     // [2 workers][heads * group] (maximum in log2 units, sum)
@@ -101,8 +103,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // What a lane holds of one unit ahead of its loads.
 struct Unit {
     int k_id, v_id;
-    int info;  // valid rows | kNewRow: the last of them is the new token
-    int bh;    // sequence * hkv + head
+    int info;  // valid rows | kNewRow: the last of them is the new token | kv head << 16
 };
 constexpr int kNewRow = 1 << 8;
 
@@ -116,7 +117,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
     constexpr int kCopies = kPageSlots / kRowsPerCopy;
     constexpr int kSteps = D / 16;
     static_assert(kStages >= 2, "the ring holds one unit ahead");
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = raw_smem + (kRingAlign - smem_addr(raw_smem) % kRingAlign) % kRingAlign;
     __shared__ int warp_sums[32];
     __shared__ int stage_info[WARPS][kStages];
     int* base = reinterpret_cast<int*>(smem + kRingBytes);
@@ -130,11 +132,109 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
     scan_counts(v.batch, base, warp_sums,
                 [&](int b) { return min(n_list, pages_of(attended(v, p.d, b, blockIdx.x == 0))); });
     const int total = base[v.batch] * p.s.groups;
-    const int per = max(p.min_units, (total + p.s.workers - 1) / p.s.workers);
+    const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
     if (blockIdx.x == 0)
         for (int b = tid; b <= v.batch; b += blockDim.x) p.base[b] = base[b];
 
     const int hq = p.d.n_q_heads;
+    const int worker = blockIdx.x * p.s.lanes + warp / p.s.heads;
+    const int head_in = warp % p.s.heads;
+    // A worker without units still helps with the appends.
+    const int64_t first = warp < p.s.lanes * p.s.heads ? min((int64_t)total, (int64_t)worker * per) : total;
+    const int u0 = (int)first, u1 = (int)min((int64_t)total, first + per);
+
+    const uint64_t policy = l2_policy_evict_first();
+    uint8_t* ring = smem + warp * (kStages * 2 * kTile);
+    const uint32_t ring_addr = smem_addr(ring);
+    const size_t slot_stride = (size_t)v.hkv * D;
+
+    // This lane's unit of the 32 from `from` on.
+    auto fetch = [&](int from) {
+        Unit n{0, 0, 0};
+        const int u = from + lane;
+        if (u >= u1) return n;
+        const int b = owner(base, v.batch, p.s.groups, u);
+        const int count = base[b + 1] - base[b];
+        const int r = u - base[b] * p.s.groups;
+        const int grp = r / count, j = r - grp * count;
+        const int h = grp * p.s.heads + head_in;
+        if (h >= v.hkv) return n;
+        const int tokens = attended(v, p.d, b, false);
+        const int lp = p.d.pages ? p.d.pages[((size_t)b * v.hkv + h) * p.d.n_pages + j] : j;
+        if (lp < 0 || lp >= pages_of(tokens)) return n;
+        const int2 e = v.table[b * v.table_stride + lp];
+        if (e.x < 0 || e.x >= v.pool_pages || e.y < 0 || e.y >= v.pool_pages) {
+            atomicOr(v.err, kErrBadPage);
+            return n;
+        }
+        n.k_id = e.x;
+        n.v_id = e.y;
+        n.info = min(kPageSlots, tokens - lp * kPageSlots) | h << 16;
+        int pos;
+        if (gains(v, p.d, b, &pos) && pos / kPageSlots == lp) n.info |= kNewRow;
+        return n;
+    };
+
+    Unit cur = fetch(u0), next = fetch(u0 + 32);
+    int cur_from = u0;
+    const int c16 = lane % kChunks, r0 = lane / kChunks;
+    // This lane's 16 bytes of the first rows of a unit: in the page, and in the
+    // ring, where row r holds chunk c at c ^ (r & 7).
+    const uint32_t lane_src = (uint32_t)(r0 * v.hkv * kRow + c16 * 16);
+    const uint32_t lane_dst = (uint32_t)(r0 * kRow + ((c16 ^ r0) << 4));
+    const uint32_t row_step = (uint32_t)(kRowsPerCopy * v.hkv * kRow);
+    int issue_at = 0, issue_stage = 0;  // units issued, and the stage of the next
+
+    auto issue = [&]() {
+        const int u = u0 + issue_at;
+        if (u < u1) {
+            if (u - cur_from >= 32) {
+                cur = next;
+                cur_from += 32;
+                next = fetch(cur_from + 32);
+            }
+            const int from = u - cur_from;
+            const int k_id = __shfl_sync(0xFFFFFFFFu, cur.k_id, from), v_id = __shfl_sync(0xFFFFFFFFu, cur.v_id, from);
+            const int info = __shfl_sync(0xFFFFFFFFu, cur.info, from);
+            const int h = info >> 16, valid = info & 0xFF;
+            if (lane == 0) stage_info[warp][issue_stage] = valid;
+            const uint32_t dst = ring_addr + issue_stage * (2 * kTile) + lane_dst;
+            const char* k = reinterpret_cast<const char*>(v.k_base) + ((size_t)k_id * (kPageSlots * v.hkv) + h) * kRow + lane_src;
+            const char* vv = reinterpret_cast<const char*>(v.v_base) + ((size_t)v_id * (kPageSlots * v.hkv) + h) * kRow + lane_src;
+            if ((info & 0xFFFF) == kPageSlots) {
+#pragma unroll
+                for (int i = 0; i < kCopies; ++i) {
+                    const uint32_t to = (dst ^ (((i * kRowsPerCopy) & 7) << 4)) + i * (kRowsPerCopy * kRow);
+                    cp_async16(to, k + (size_t)i * row_step, 16u, policy);
+                    cp_async16(to + kTile, vv + (size_t)i * row_step, 16u, policy);
+                }
+            } else {
+                const int b = owner(base, v.batch, p.s.groups, u);
+#pragma unroll 1
+                for (int i = 0; i < kCopies; ++i) {
+                    const int row = i * kRowsPerCopy + r0;
+                    const uint32_t to = (dst ^ (((i * kRowsPerCopy) & 7) << 4)) + i * (kRowsPerCopy * kRow);
+                    const void* ks = k + (size_t)i * row_step;
+                    const void* vs = vv + (size_t)i * row_step;
+                    if ((info & kNewRow) && row == valid - 1) {
+                        ks = p.d.k_new + b * p.d.k_stride_batch + h * p.d.k_stride_head + c16 * 8;
+                        vs = p.d.v_new + b * p.d.v_stride_batch + h * p.d.v_stride_head + c16 * 8;
+                    }
+                    // Rows behind the sequence become zeros: what the slots hold may be anything.
+                    const uint32_t bytes = row < valid ? 16u : 0u;
+                    cp_async16(to, ks, bytes, policy);
+                    cp_async16(to + kTile, vs, bytes, policy);
+                }
+            }
+            ++issue_at;
+            if (++issue_stage == kStages) issue_stage = 0;
+        }
+        cp_async_commit();
+    };
+
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) issue();
+
     for (int b = blockIdx.x; b < v.batch; b += gridDim.x) {
         // The new token's rows go to their page slot; its readers below take
         // them from the step's inputs, so neither waits for the other.
@@ -163,96 +263,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
         }
     }
 
-    const int worker = blockIdx.x * p.s.lanes + warp / p.s.heads;
-    const int head_in = warp % p.s.heads;
-    if (warp >= p.s.lanes * p.s.heads) return;
-    const int64_t first = (int64_t)worker * per;
-    if (first >= total) return;
-    const int u0 = (int)first, u1 = (int)min((int64_t)total, first + per);
-
-    const uint64_t policy = l2_policy_evict_first();
-    uint8_t* ring = smem + warp * (kStages * 2 * kTile);
-    const uint32_t ring_addr = smem_addr(ring);
-    const size_t slot_stride = (size_t)v.hkv * D;
-
-    // This lane's unit of the 32 from `from` on.
-    auto fetch = [&](int from) {
-        Unit n{0, 0, 0, 0};
-        const int u = from + lane;
-        if (u >= u1) return n;
-        const int b = owner(base, v.batch, p.s.groups, u);
-        const int count = base[b + 1] - base[b];
-        const int r = u - base[b] * p.s.groups;
-        const int grp = r / count, j = r - grp * count;
-        const int h = grp * p.s.heads + head_in;
-        if (h >= v.hkv) return n;
-        const int tokens = attended(v, p.d, b, false);
-        n.bh = b * v.hkv + h;
-        const int lp = p.d.pages ? p.d.pages[(size_t)n.bh * p.d.n_pages + j] : j;
-        if (lp < 0 || lp >= pages_of(tokens)) return n;
-        const int2 e = v.table[b * v.table_stride + lp];
-        if (e.x < 0 || e.x >= v.pool_pages || e.y < 0 || e.y >= v.pool_pages) {
-            atomicOr(v.err, kErrBadPage);
-            return n;
-        }
-        n.k_id = e.x;
-        n.v_id = e.y;
-        n.info = min(kPageSlots, tokens - lp * kPageSlots);
-        int pos;
-        if (gains(v, p.d, b, &pos) && pos / kPageSlots == lp) n.info |= kNewRow;
-        return n;
-    };
-
-    Unit cur = fetch(u0), next = fetch(u0 + 32);
-    int cur_from = u0;
-    const int c16 = lane % kChunks, r0 = lane / kChunks;
-
-    auto issue = [&](int u) {
-        if (u < u1) {
-            if (u - cur_from >= 32) {
-                cur = next;
-                cur_from += 32;
-                next = fetch(cur_from + 32);
-            }
-            const int from = u - cur_from;
-            const int k_id = __shfl_sync(0xFFFFFFFFu, cur.k_id, from), v_id = __shfl_sync(0xFFFFFFFFu, cur.v_id, from);
-            const int info = __shfl_sync(0xFFFFFFFFu, cur.info, from), bh = __shfl_sync(0xFFFFFFFFu, cur.bh, from);
-            const int h = bh % v.hkv, valid = info & 0xFF;
-            const int stage = (u - u0) % kStages;
-            if (lane == 0) stage_info[warp][stage] = valid;
-            const uint32_t dst = ring_addr + stage * (2 * kTile);
-            const uint16_t* k = v.k_base + ((size_t)k_id * kPageSlots + r0) * slot_stride + h * D + c16 * 8;
-            const uint16_t* vv = v.v_base + ((size_t)v_id * kPageSlots + r0) * slot_stride + h * D + c16 * 8;
-            const bool has_new = info & kNewRow;
-#pragma unroll
-            for (int i = 0; i < kCopies; ++i) {
-                const int row = i * kRowsPerCopy + r0;
-                const uint32_t to = dst + row * kRow + ((c16 ^ (row & 7)) << 4);
-                const uint16_t* ks = k + i * kRowsPerCopy * slot_stride;
-                const uint16_t* vs = vv + i * kRowsPerCopy * slot_stride;
-                if (has_new && row == valid - 1) {
-                    const int b = bh / v.hkv;
-                    ks = p.d.k_new + b * p.d.k_stride_batch + h * p.d.k_stride_head + c16 * 8;
-                    vs = p.d.v_new + b * p.d.v_stride_batch + h * p.d.v_stride_head + c16 * 8;
-                }
-                // Rows behind the sequence become zeros: what the slots hold may be anything.
-                const uint32_t bytes = row < valid ? 16u : 0u;
-                cp_async16(to, ks, bytes, policy);
-                cp_async16(to + kTile, vs, bytes, policy);
-            }
-        }
-        cp_async_commit();
-    };
-
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(u0 + i);
-
     const int g4 = lane >> 2, c2 = (lane & 3) * 2;  // fragment row, first column
-    const int k_row = lane & 15, k_chunk = lane >> 4;
-    const int v_row = (lane & 7) + ((lane >> 4) << 3), v_chunk = (lane >> 3) & 1;
+    // This lane's row and first chunk for ldmatrix; step i is 2 i chunks on, which
+    // under the permutation is an XOR (tiles start on multiples of their row).
+    const int k_row = lane & 15, v_row = (lane & 7) + ((lane >> 4) << 3);
+    const uint32_t k_at = k_row * kRow + (((lane >> 4) ^ (k_row & 7)) << 4);
+    const uint32_t v_at = v_row * kRow + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
     const int G = p.group;
 
-    int u = u0;
+    int u = u0, read_stage = 0;
     while (u < u1) {
         // One segment: the rest of (sequence, head group) inside [u, u1).
         const int b = owner(base, v.batch, p.s.groups, u);
@@ -293,8 +312,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
         for (; u < end; ++u) {
             cp_async_wait<kStages - 2>();
             __syncwarp();
-            issue(u + kStages - 1);
-            const int stage = (u - u0) % kStages;
+            issue();
+            const int stage = read_stage;
+            if (++read_stage == kStages) read_stage = 0;
             const int valid = stage_info[warp][stage];
             if (valid == 0) {
                 // A skipped page gets no weight.
@@ -305,16 +325,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
             any_key = true;
             const uint32_t tile = ring_addr + stage * (2 * kTile);
 
-            float s[NT][4];
+            float s[NT][4], odd[NT][4];  // two chains of products
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] = odd[nt][i] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) {
                 uint32_t a[4];
-                ldmatrix4(a, tile + k_row * kRow + (((2 * ks + k_chunk) ^ (k_row & 7)) << 4));
+                ldmatrix4(a, (tile + k_at) ^ (ks * 32));
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816<F16>(s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+                for (int nt = 0; nt < NT; ++nt) mma16816<F16>(ks & 1 ? odd[nt] : s[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] += odd[nt][i];
             uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -371,7 +397,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
                 uint32_t a[4];
-                ldmatrix4_trans(a, tile + kTile + v_row * kRow + (((2 * i + v_chunk) ^ (v_row & 7)) << 4));
+                ldmatrix4_trans(a, (tile + kTile + v_at) ^ (i * 32));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma16816<F16>(acc[nt][i], a, hi[nt][0], hi[nt][1]);
@@ -422,66 +448,134 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
     }
 }
 
-// Joins the parts of each cut sequence, in order: block (segment, row), the
-// row one of the group's query heads; eight warps take the parts in turn.
-constexpr int kJoinWarps = 8;
+// Joins the parts of each cut sequence, in order. An item is (segment, y): a
+// segment of at most 32 parts is joined by its first items, one row (query
+// head) a warp; a longer one by all, one row a CTA, its warps taking the parts
+// in turn. Either way the factors of all parts come first, so that the loads
+// of their outputs depend on nothing. (Folding with a running maximum, one
+// warp after the other, took 13 us on 147 parts; this takes 5.)
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
 template <int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) batch_join_kernel(const DecodeParams p) {
-    constexpr int kPer = D / 32;
+__global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(const DecodeParams p) {
+    constexpr int kPer = D / 32;  // dims of a lane
+    constexpr int kBatch = 8;     // parts of a warp in flight
+    constexpr int kFactors = kMaxGrid * 8;
+    constexpr int kRounds = (kFactors + kJoinThreads - 1) / kJoinThreads;
+    __shared__ float factor[kFactors];  // of all parts
     __shared__ float sh_acc[kJoinWarps][D];
     __shared__ float2 sh_ml[kJoinWarps];
     pdl_wait();
     pdl_trigger();
-    const int total = p.base[p.v.batch] * p.s.groups;
-    const int per = max(p.min_units, (total + p.s.workers - 1) / p.s.workers);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows = p.s.heads * p.group;
-    for (int seg = blockIdx.x; seg < p.v.batch * p.s.groups; seg += gridDim.x) {
+    const int segments = p.v.batch * p.s.groups;
+    const int total = p.base[p.v.batch] * p.s.groups;
+    const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
+    for (int64_t item = blockIdx.x; item < (int64_t)segments * rows; item += gridDim.x) {
+        const int y = (int)(item / segments), seg = (int)(item - (int64_t)y * segments);
         const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
-        const int count = p.base[b + 1] - p.base[b];
+        const int base = p.base[b], count = p.base[b + 1] - base;
         if (count == 0) continue;
-        const int s0 = p.base[b] * p.s.groups + grp * count, s1 = s0 + count;
-        const int w0 = s0 / per, w1 = (s1 - 1) / per;
-        if (w0 == w1) continue;
-        const int head = grp * p.s.heads + (int)blockIdx.y / p.group;
-        if (head >= p.v.hkv) continue;
-        float m = -INFINITY, l = 0.f, acc[kPer];
+        const int s0 = base * p.s.groups + grp * count, s1 = s0 + count;
+        const int w0 = s0 / per, w1 = (s1 - 1) / per, parts = w1 - w0 + 1;
+        if (parts == 1) continue;
+        const bool one_warp = parts <= 32;
+        const int row = one_warp ? y * kJoinWarps + warp : y;
+        const bool there = row < rows && grp * p.s.heads + row / p.group < p.v.hkv;
+        // Part i lies in its worker's first slot, the segment's first part in the second unless it starts the worker's.
+        auto slot = [&](int i) {
+            return (size_t)(2 * (w0 + i) + (i == 0 && s0 != w0 * per ? 1 : 0)) * rows + row;
+        };
+        // The sum of parts first, first + step, .. of this row, their factors given.
+        float acc[kPer];
+        auto sum_parts = [&](int first, int step, auto factor_of) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] = 0.f;
-        for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
-            const size_t slot = (size_t)(2 * w + (w == w0 && s0 != w0 * per ? 1 : 0)) * rows + blockIdx.y;
-            const float2 ml = p.part_ml[slot];
-            const float n = fmaxf(m, ml.x);
-            const float a = n == m ? 1.f : exp2_of(m - n), c = n == ml.x ? 1.f : exp2_of(ml.x - n);
-            m = n;
-            l = l * a + ml.y * c;
+            for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+            for (int i = first; i < parts; i += step * kBatch) {
+                float x[kBatch][kPer], c[kBatch];
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * a + p.part_acc[slot * D + i * 32 + lane] * c;
+                for (int k = 0; k < kBatch; ++k) {
+                    const int at = i + k * step;
+                    c[k] = factor_of(min(at, parts - 1));
+                    const float* from = p.part_acc + slot(min(at, parts - 1)) * D + lane;
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) x[k][j] = at < parts ? from[j * 32] : 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) acc[j] += x[k][j] * c[k];
+            }
+        };
+        const size_t q_row = (size_t)b * p.d.n_q_heads + grp * rows + row;
+        if (one_warp) {
+            if (!there) continue;
+            const float2 ml = lane < parts ? p.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+            float m = ml.x;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+            const float c = ml.x == m ? 1.f : exp2_of(ml.x - m);
+            float l = ml.y * c;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+            sum_parts(0, 1, [&](int i) { return __shfl_sync(~0u, c, i); });
+            const bool none = m == -INFINITY;  // no key at all
+            const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) store_out(p.d.out, q_row * D + j * 32 + lane, acc[j] * inv, p.d.out_dtype);
+            if (lane == 0) {
+                const float e = none ? -INFINITY : m + log2f(l);
+                p.lse2[q_row] = e;
+                if (p.d.lse) p.d.lse[q_row] = e * kLn2;
+            }
+            continue;
         }
-        if (lane == 0) sh_ml[warp] = make_float2(m, l);
+        if (!there) continue;
+        float m = -INFINITY;
+        float2 ml[kRounds];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sh_acc[warp][i * 32 + lane] = acc[i];
+        for (int k = 0; k < kRounds; ++k) {
+            const int i = k * kJoinThreads + threadIdx.x;
+            ml[k] = i < parts ? p.part_ml[slot(i)] : make_float2(-INFINITY, 0.f);
+            m = fmaxf(m, ml[k].x);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        if (lane == 0) sh_ml[warp].x = m;
         __syncthreads();
-        float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) M = fmaxf(M, sh_ml[w].x);
-        float c[kJoinWarps];
+        for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sh_ml[w].x);
+        float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
-            c[w] = sh_ml[w].x == M ? 1.f : exp2_of(sh_ml[w].x - M);
-            L += sh_ml[w].y * c[w];
+        for (int k = 0; k < kRounds; ++k) {
+            const int i = k * kJoinThreads + threadIdx.x;
+            if (i < parts) {
+                const float c = ml[k].x == m ? 1.f : exp2_of(ml[k].x - m);
+                factor[i] = c;
+                l += ml[k].y * c;
+            }
         }
-        const size_t q_row = (size_t)b * p.d.n_q_heads + grp * rows + blockIdx.y;
-        const bool none = M == -INFINITY;  // no key at all
-        const float inv = none ? 0.f : 1.f / L;
-        for (int d = threadIdx.x; d < D; d += blockDim.x) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+        if (lane == 0) sh_ml[warp].y = l;
+        __syncthreads();
+        sum_parts(warp, kJoinWarps, [&](int i) { return factor[i]; });
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) sh_acc[warp][j * 32 + lane] = acc[j];
+        __syncthreads();
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) l += sh_ml[w].y;
+        const bool none = m == -INFINITY;
+        const float inv = none ? 0.f : 1.f / l;
+        for (int d = threadIdx.x; d < D; d += kJoinThreads) {
             float o = 0.f;
 #pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) o += sh_acc[w][d] * c[w];
+            for (int w = 0; w < kJoinWarps; ++w) o += sh_acc[w][d];
             store_out(p.d.out, q_row * D + d, o * inv, p.d.out_dtype);
         }
         if (threadIdx.x == 0) {
-            const float e = none ? -INFINITY : M + log2f(L);
+            const float e = none ? -INFINITY : m + log2f(l);
             p.lse2[q_row] = e;
             if (p.d.lse) p.d.lse[q_row] = e * kLn2;
         }
@@ -489,29 +583,41 @@ __global__ void __launch_bounds__(kJoinWarps * 32) batch_join_kernel(const Decod
     }
 }
 
-// weights_out[t] = decay * weights_in[t] + sum over the head's queries of exp2(s_t - lse).
-__global__ void __launch_bounds__(256) batch_totals_kernel(const DecodeParams p) {
+// weights_out[t] = decay * weights_in[t] + sum over the head's queries of
+// exp2(s_t - lse): a thread per token, over a line of 256-token chunks of all
+// (sequence, head) rows. Bound: HBM and L2, 4 G + 8 bytes a token and head.
+constexpr int kTotalsThreads = 256;
+__global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const DecodeParams p) {
+    extern __shared__ int chunks[];
+    __shared__ int warp_sums[32];
     pdl_wait();
     pdl_trigger();
-    const int b = blockIdx.z, h = blockIdx.y;
-    const int n = attended(p.v, p.d, b, false);
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    const int G = p.group;
-    const int count = p.base[b + 1] - p.base[b];
-    const float* s = p.scores + (((size_t)p.base[b] * p.v.hkv + (size_t)h * count) * kPageSlots + t) * G;
-    const float* e = p.lse2 + (size_t)b * p.d.n_q_heads + h * G;
-    float sum = 0.f;
-    for (int g = 0; g < G; ++g) sum += exp2_of(s[g] - e[g]);
-    const size_t at = ((size_t)b * p.v.hkv + h) * p.d.weights_stride + t;
-    const bool old = p.d.weights_in && t < p.v.lens[b];
-    p.d.weights_out[at] = old ? p.d.decay * p.d.weights_in[at] + sum : sum;
+    const int G = p.group, hkv = p.v.hkv;
+    constexpr int kPages = kTotalsThreads / kPageSlots;
+    scan_counts(p.v.batch, chunks, warp_sums,
+                [&](int b) { return (p.base[b + 1] - p.base[b] + kPages - 1) / kPages; });
+    const int64_t all = (int64_t)chunks[p.v.batch] * hkv;
+    for (int64_t c = blockIdx.x; c < all; c += gridDim.x) {
+        const int at = (int)(c / hkv), h = (int)(c - (int64_t)at * hkv);
+        const int b = owner(chunks, p.v.batch, 1, at);
+        const int t = (at - chunks[b]) * kTotalsThreads + threadIdx.x;
+        const int n = attended(p.v, p.d, b, false);
+        if (t >= n) continue;
+        const int base = p.base[b], count = p.base[b + 1] - base;
+        const size_t place = ((size_t)b * hkv + h) * p.d.weights_stride + t;
+        const float old = p.d.weights_in && t < p.v.lens[b] ? p.d.decay * p.d.weights_in[place] : 0.f;
+        const float* s = p.scores + (((size_t)base * hkv + (size_t)h * count) * kPageSlots + t) * G;
+        const float* e = p.lse2 + (size_t)b * p.d.n_q_heads + h * G;
+        float sum = 0.f;
+        for (int g = 0; g < G; ++g) sum += exp2_of(s[g] - e[g]);
+        p.d.weights_out[place] = old + sum;
+    }
 }
 
 template <int D>
 constexpr int warps_of() { return D == 256 ? 4 : 8; }
 
-size_t smem_bytes(int batch) { return kRingBytes + sizeof(int) * (size_t)(batch + 1); }
+size_t smem_bytes(int batch) { return kRingAlign + kRingBytes + sizeof(int) * (size_t)(batch + 1); }
 
 template <typename F>
 cudaError_t for_kernel(bool f16, int dim, bool two, F f) {
@@ -558,7 +664,7 @@ BatchSplit batch_split(const BatchView& v) {
     s.heads = v.hkv < s.warps ? v.hkv : s.warps;
     s.groups = (v.hkv + s.heads - 1) / s.heads;
     s.lanes = s.warps / s.heads;
-    s.grid = v.sms;
+    s.grid = v.sms < kMaxGrid ? v.sms : kMaxGrid;
     s.workers = s.grid * s.lanes;
     return s;
 }
@@ -586,7 +692,6 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
     p.d = d;
     p.s = batch_split(v);
     p.group = d.n_q_heads / v.hkv;
-    p.min_units = kMinUnits;
     p.scale_log2 = d.scale * kLog2e;
     const DecodeSpace o = decode_space(v, p.s, d.n_q_heads, d.weights_out != nullptr);
     char* w = static_cast<char*>(d.workspace);
@@ -601,14 +706,14 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
     if (e != cudaSuccess) return e;
     // The join is always launched: it also keeps the launches behind it from
     // starting before the appended rows are in their pages.
-    const int segments = v.batch * p.s.groups;
-    const dim3 grid(segments < 65535 ? segments : 65535, p.s.heads * p.group);
-    e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinWarps * 32), 0, stream, p)
-        : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinWarps * 32), 0, stream, p)
-                       : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinWarps * 32), 0, stream, p);
+    const int64_t items = (int64_t)v.batch * p.s.groups * p.s.heads * p.group;
+    const dim3 grid((unsigned)std::min<int64_t>(items, (int64_t)v.sms * 8));
+    e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinThreads), 0, stream, p)
+        : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinThreads), 0, stream, p)
+                       : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinThreads), 0, stream, p);
     if (e != cudaSuccess || !d.weights_out) return e;
-    return launch_dependent(batch_totals_kernel, dim3((v.table_pages * kPageSlots + 255) / 256, v.hkv, v.batch),
-                            dim3(256), 0, stream, p);
+    return launch_dependent(batch_totals_kernel, dim3(v.sms * 8), dim3(kTotalsThreads),
+                            sizeof(int) * (size_t)(v.batch + 1), stream, p);
 }
 
 }  // namespace gkv
