@@ -17,6 +17,19 @@ __device__ __forceinline__ int pages_of(int n) { return (n + kPageSlots - 1) / k
 template <typename Count>
 __device__ __forceinline__ void scan_counts(int batch, int* base, int* warp_sums, Count count) {
     const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31;
+    if (batch <= 32) {
+        // Every warp for itself: the same values, no barrier.
+        int inc = lane < batch ? count(lane) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        if (lane < batch) base[lane + 1] = inc;
+        if (lane == 0) base[0] = 0;
+        __syncwarp();
+        return;
+    }
     const int run = (batch + n - 1) / n;
     const int b0 = min(batch, tid * run), b1 = min(batch, b0 + run);
     int sum = 0;

@@ -42,7 +42,6 @@ struct DecodeParams {
     float* part_acc;     // [2 workers][heads * group][D]
     float2* part_ml;     // [2 workers][heads * group] (maximum in log2 units, sum)
     float* lse2;         // [batch][Hq] log2 of the sum, for the totals
-    int32_t* base;       // [batch + 1] units before each sequence
     float* scores;       // [unit][16][group] scores in log2 units, for the totals; or null
 };
 
@@ -100,10 +99,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return r;
 }
 
-// What a lane holds of one unit ahead of its loads.
+// What a lane holds of one unit ahead of its loads. The ids stay unchecked
+// until they are used, so that a load of 32 of them is not waited for.
 struct Unit {
-    int k_id, v_id;
-    int info;  // valid rows | kNewRow: the last of them is the new token | kv head << 16
+    int2 ids;
+    int info;  // valid rows | kNewRow: the last of them is the new token | kv head << 16; 0: no page
 };
 constexpr int kNewRow = 1 << 8;
 
@@ -125,16 +125,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
 
     const BatchView& v = p.v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_trigger();
     pdl_wait();
+    // From here on the kernels behind may start: they read lengths and inputs
+    // before this one is done, the workspace only after.
+    pdl_trigger();
 
     const int n_list = p.d.pages ? p.d.n_pages : 0x7FFFFFFF;
     scan_counts(v.batch, base, warp_sums,
                 [&](int b) { return min(n_list, pages_of(attended(v, p.d, b, blockIdx.x == 0))); });
     const int total = base[v.batch] * p.s.groups;
     const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
-    if (blockIdx.x == 0)
-        for (int b = tid; b <= v.batch; b += blockDim.x) p.base[b] = base[b];
 
     const int hq = p.d.n_q_heads;
     const int worker = blockIdx.x * p.s.lanes + warp / p.s.heads;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
 
     // This lane's unit of the 32 from `from` on.
     auto fetch = [&](int from) {
-        Unit n{0, 0, 0};
+        Unit n{make_int2(0, 0), 0};
         const int u = from + lane;
         if (u >= u1) return n;
         const int b = owner(base, v.batch, p.s.groups, u);
@@ -162,20 +162,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
         const int tokens = attended(v, p.d, b, false);
         const int lp = p.d.pages ? p.d.pages[((size_t)b * v.hkv + h) * p.d.n_pages + j] : j;
         if (lp < 0 || lp >= pages_of(tokens)) return n;
-        const int2 e = v.table[b * v.table_stride + lp];
-        if (e.x < 0 || e.x >= v.pool_pages || e.y < 0 || e.y >= v.pool_pages) {
-            atomicOr(v.err, kErrBadPage);
-            return n;
-        }
-        n.k_id = e.x;
-        n.v_id = e.y;
+        n.ids = v.table[b * v.table_stride + lp];
         n.info = min(kPageSlots, tokens - lp * kPageSlots) | h << 16;
         int pos;
         if (gains(v, p.d, b, &pos) && pos / kPageSlots == lp) n.info |= kNewRow;
         return n;
     };
 
-    Unit cur = fetch(u0), next = fetch(u0 + 32);
+    auto checked = [&](Unit n) {
+        if (n.info && (min(n.ids.x, n.ids.y) < 0 || max(n.ids.x, n.ids.y) >= v.pool_pages)) {
+            atomicOr(v.err, kErrBadPage);
+            n.info = 0;
+        }
+        if (!n.info) n.ids = make_int2(0, 0);
+        return n;
+    };
+
+    Unit cur = checked(fetch(u0)), next;
     int cur_from = u0;
     const int c16 = lane % kChunks, r0 = lane / kChunks;
     // This lane's 16 bytes of the first rows of a unit: in the page, and in the
@@ -189,12 +192,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
         const int u = u0 + issue_at;
         if (u < u1) {
             if (u - cur_from >= 32) {
-                cur = next;
+                cur = checked(next);
                 cur_from += 32;
                 next = fetch(cur_from + 32);
             }
             const int from = u - cur_from;
-            const int k_id = __shfl_sync(0xFFFFFFFFu, cur.k_id, from), v_id = __shfl_sync(0xFFFFFFFFu, cur.v_id, from);
+            const int k_id = __shfl_sync(0xFFFFFFFFu, cur.ids.x, from), v_id = __shfl_sync(0xFFFFFFFFu, cur.ids.y, from);
             const int info = __shfl_sync(0xFFFFFFFFu, cur.info, from);
             const int h = info >> 16, valid = info & 0xFF;
             if (lane == 0) stage_info[warp][issue_stage] = valid;
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
 
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) issue();
+    next = fetch(u0 + 32);
 
     for (int b = blockIdx.x; b < v.batch; b += gridDim.x) {
         // The new token's rows go to their page slot; its readers below take
@@ -271,33 +275,64 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
     const uint32_t v_at = v_row * kRow + ((((lane >> 3) & 1) ^ (v_row & 7)) << 4);
     const int G = p.group;
 
-    int u = u0, read_stage = 0;
-    while (u < u1) {
-        // One segment: the rest of (sequence, head group) inside [u, u1).
-        const int b = owner(base, v.batch, p.s.groups, u);
-        const int count = base[b + 1] - base[b];
-        const int seq0 = base[b] * p.s.groups;
-        const int grp = (u - seq0) / count;
-        const int seg0 = seq0 + grp * count, seg1 = seg0 + count;
-        const int begin = u, end = min(u1, seg1);
-        const int h = grp * p.s.heads + head_in;
-        const bool mine = h < v.hkv;
-        float* score_row = p.scores && mine
-                               ? p.scores + ((size_t)base[b] * v.hkv + (size_t)h * count) * (kPageSlots * G)
-                               : nullptr;
-
-        // Q of the segment as B fragments (16 dims x 8 heads).
-        uint32_t qf[NT][kSteps][2];
+    // A segment is what a worker has of one (sequence, head group): units
+    // [begin, end) of the group's [seg0, seg1).
+    struct Segment {
+        int b, h, base, count, seg0, begin, end;
+        bool mine;  // the last group may have fewer heads than warps
+    };
+    auto segment_at = [&](int u) {
+        Segment g;
+        g.b = owner(base, v.batch, p.s.groups, u);
+        g.base = base[g.b];
+        g.count = base[g.b + 1] - g.base;
+        const int grp = (u - g.base * p.s.groups) / g.count;
+        g.seg0 = g.base * p.s.groups + grp * g.count;
+        g.begin = u;
+        g.end = min(u1, g.seg0 + g.count);
+        g.h = grp * p.s.heads + head_in;
+        g.mine = g.h < v.hkv;
+        return g;
+    };
+    // Q of a segment as B fragments (16 dims x 8 heads). With few query heads the
+    // next segment's come in while this one's pages do.
+    auto load_q = [&](const Segment& sg, uint32_t (&qf)[NT][kSteps][2]) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int g = nt * 8 + g4;
-            const uint16_t* row = p.d.q + b * p.d.q_stride_batch + (int64_t)(h * G + g) * p.d.q_stride_head + c2;
+            const bool there = sg.mine && g < G;
+            const uint16_t* row = p.d.q + sg.b * p.d.q_stride_batch + (int64_t)(sg.h * G + g) * p.d.q_stride_head + c2;
 #pragma unroll
             for (int ks = 0; ks < kSteps; ++ks) {
-                qf[nt][ks][0] = mine && g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
-                qf[nt][ks][1] = mine && g < G ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
+                qf[nt][ks][0] = there ? *reinterpret_cast<const uint32_t*>(row + ks * 16) : 0u;
+                qf[nt][ks][1] = there ? *reinterpret_cast<const uint32_t*>(row + ks * 16 + 8) : 0u;
             }
         }
+    };
+    constexpr bool kAhead = NT == 1 && D <= 128;
+
+    int u = u0, read_stage = 0;
+    Segment sg{}, sg_next{};
+    uint32_t qf[NT][kSteps][2], q_next[NT][kSteps][2];
+    if (u0 < u1) {
+        sg_next = segment_at(u0);
+        load_q(sg_next, q_next);
+    }
+    while (u < u1) {
+        sg = sg_next;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int ks = 0; ks < kSteps; ++ks) qf[nt][ks][0] = q_next[nt][ks][0], qf[nt][ks][1] = q_next[nt][ks][1];
+        if (sg.end < u1) {
+            sg_next = segment_at(sg.end);
+            if (kAhead) load_q(sg_next, q_next);
+        }
+        const int b = sg.b, h = sg.h, seg0 = sg.seg0, seg1 = sg.seg0 + sg.count, begin = sg.begin, end = sg.end;
+        const bool mine = sg.mine;
+        float* score_row = p.scores && mine
+                               ? p.scores + ((size_t)sg.base * v.hkv + (size_t)h * sg.count) * (kPageSlots * G)
+                               : nullptr;
         float acc[NT][kSteps][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
@@ -405,6 +440,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
                 }
             }
         }
+        if (!kAhead && sg.end < u1) load_q(sg_next, q_next);
         if (!mine) continue;
 
         const bool whole = begin == seg0 && end == seg1;
@@ -412,104 +448,134 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
         const size_t slot = (size_t)(2 * worker + (begin == u0 ? 0 : 1)) * rows + head_in * G;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            float inv[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][i], o);
+                inv[i] = any_key ? 1.f / l[nt][i] : 0.f;
                 const int g = nt * 8 + c2 + i;
-                if (g >= G) continue;
-                const size_t q_row = (size_t)b * hq + h * G + g;
+                if (g4 != 0 || g >= G) continue;
                 if (whole) {
-                    const float inv = any_key ? 1.f / l[nt][i] : 0.f;
-                    if (g4 == 0) {
-                        const float e = any_key ? m[nt][i] + log2f(l[nt][i]) : -INFINITY;
-                        p.lse2[q_row] = e;
-                        if (p.d.lse) p.d.lse[q_row] = e * kLn2;
-                    }
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        store_out(p.d.out, q_row * D + k * 16 + g4, acc[nt][k][i] * inv, p.d.out_dtype);
-                        store_out(p.d.out, q_row * D + k * 16 + g4 + 8, acc[nt][k][i + 2] * inv, p.d.out_dtype);
-                    }
+                    const float e = any_key ? m[nt][i] + log2f(l[nt][i]) : -INFINITY;
+                    const size_t q_row = (size_t)b * hq + h * G + g;
+                    p.lse2[q_row] = e;
+                    if (p.d.lse) p.d.lse[q_row] = e * kLn2;
                 } else {
                     // A part whose scores were all -inf is told from one without keys by its maximum.
-                    if (g4 == 0)
-                        p.part_ml[slot + g] =
-                            make_float2(any_key && m[nt][i] == -INFINITY ? kLowest : m[nt][i], l[nt][i]);
-                    float* to = p.part_acc + (slot + g) * D + g4;
+                    p.part_ml[slot + g] = make_float2(any_key && m[nt][i] == -INFINITY ? kLowest : m[nt][i], l[nt][i]);
+                }
+            }
+            if (whole && p.d.out_dtype != 0) {
+                // Transposed, so that a lane holds two neighbouring dims of one head.
+                uint16_t* to = static_cast<uint16_t*>(p.d.out) + ((size_t)b * hq + h * G + nt * 8 + g4) * D + c2;
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        to[k * 16] = acc[nt][k][i];
-                        to[k * 16 + 8] = acc[nt][k][i + 2];
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const float x = acc[nt][k][half * 2] * inv[0], y = acc[nt][k][half * 2 + 1] * inv[1];
+                        const uint32_t w = transpose8x8(p.d.out_dtype == 30 ? pack2<false>(x, y) : pack2<true>(x, y));
+                        if (nt * 8 + g4 < G) *reinterpret_cast<uint32_t*>(to + k * 16 + half * 8) = w;
                     }
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int g = nt * 8 + c2 + i;
+                if (g >= G) continue;
+                const float factor = whole ? inv[i] : 1.f;
+                float* to = (whole ? static_cast<float*>(p.d.out) + ((size_t)b * hq + h * G) * D : p.part_acc + slot * D) +
+                            (size_t)g * D + g4;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    to[k * 16] = acc[nt][k][i] * factor;
+                    to[k * 16 + 8] = acc[nt][k][i + 2] * factor;
                 }
             }
         }
     }
 }
 
+// Units of sequence b, as the decode kernel counted them. The join and the
+// totals call it before their wait: the decode kernel lets them start when its
+// own predecessors are done, and nothing of this call writes the lengths (they
+// are read past L1, which may hold older ones).
+__device__ __forceinline__ int units_of(const DecodeParams& p, int b) {
+    const int len = __ldcg(p.v.lens + b);
+    if (len < 0) return 0;
+    const int tokens = min(len, p.v.table_pages * kPageSlots - (p.d.k_new ? 1 : 0)) + (p.d.k_new ? 1 : 0);
+    return min(p.d.pages ? p.d.n_pages : 0x7FFFFFFF, pages_of(tokens));
+}
+
 // Joins the parts of each cut sequence, in order. An item is (segment, y): a
 // segment of at most 32 parts is joined by its first items, one row (query
 // head) a warp; a longer one by all, one row a CTA, its warps taking the parts
-// in turn. Either way the factors of all parts come first, so that the loads
-// of their outputs depend on nothing. (Folding with a running maximum, one
-// warp after the other, took 13 us on 147 parts; this takes 5.)
+// in turn. Bound: latency, two round trips to L2 behind the wait: nothing that
+// is loaded depends on the parts' maxima. (Folding with a running maximum, one
+// warp after the other, took 13 us on 147 parts.)
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(const DecodeParams p) {
-    constexpr int kPer = D / 32;  // dims of a lane
-    constexpr int kBatch = 8;     // parts of a warp in flight
+__global__ void __launch_bounds__(kJoinThreads, 2) batch_join_kernel(const DecodeParams p) {
+    constexpr int kPer = D / 32;                  // dims of a lane, neighbours
+    constexpr int kBatch = D == 256 ? 10 : 20;    // parts of a warp in flight
     constexpr int kFactors = kMaxGrid * 8;
     constexpr int kRounds = (kFactors + kJoinThreads - 1) / kJoinThreads;
+    extern __shared__ int base[];
+    __shared__ int warp_sums[32];
     __shared__ float factor[kFactors];  // of all parts
     __shared__ float sh_acc[kJoinWarps][D];
     __shared__ float2 sh_ml[kJoinWarps];
-    pdl_wait();
-    pdl_trigger();
+    scan_counts(p.v.batch, base, warp_sums, [&](int b) { return units_of(p, b); });
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows = p.s.heads * p.group;
     const int segments = p.v.batch * p.s.groups;
-    const int total = p.base[p.v.batch] * p.s.groups;
+    const int total = base[p.v.batch] * p.s.groups;
     const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
+    pdl_wait();
+    pdl_trigger();
     for (int64_t item = blockIdx.x; item < (int64_t)segments * rows; item += gridDim.x) {
         const int y = (int)(item / segments), seg = (int)(item - (int64_t)y * segments);
         const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
-        const int base = p.base[b], count = p.base[b + 1] - base;
+        const int count = base[b + 1] - base[b];
         if (count == 0) continue;
-        const int s0 = base * p.s.groups + grp * count, s1 = s0 + count;
+        const int s0 = base[b] * p.s.groups + grp * count, s1 = s0 + count;
         const int w0 = s0 / per, w1 = (s1 - 1) / per, parts = w1 - w0 + 1;
         if (parts == 1) continue;
         const bool one_warp = parts <= 32;
         const int row = one_warp ? y * kJoinWarps + warp : y;
         const bool there = row < rows && grp * p.s.heads + row / p.group < p.v.hkv;
+        if (!there) continue;
         // Part i lies in its worker's first slot, the segment's first part in the second unless it starts the worker's.
         auto slot = [&](int i) {
             return (size_t)(2 * (w0 + i) + (i == 0 && s0 != w0 * per ? 1 : 0)) * rows + row;
         };
-        // The sum of parts first, first + step, .. of this row, their factors given.
-        float acc[kPer];
-        auto sum_parts = [&](int first, int step, auto factor_of) {
+        const int first = one_warp ? 0 : warp, step = one_warp ? 1 : kJoinWarps;
+        float x[kBatch][kPer], acc[kPer];
+        auto load = [&](int from) {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
-            for (int i = first; i < parts; i += step * kBatch) {
-                float x[kBatch][kPer], c[kBatch];
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = from + k * step;
+                const float* at = p.part_acc + slot(min(i, parts - 1)) * D + lane * kPer;
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const int at = i + k * step;
-                    c[k] = factor_of(min(at, parts - 1));
-                    const float* from = p.part_acc + slot(min(at, parts - 1)) * D + lane;
-#pragma unroll
-                    for (int j = 0; j < kPer; ++j) x[k][j] = at < parts ? from[j * 32] : 0.f;
+                for (int j = 0; j < kPer; j += 2) {
+                    const float2 v2 = i < parts ? *reinterpret_cast<const float2*>(at + j) : make_float2(0.f, 0.f);
+                    x[k][j] = v2.x, x[k][j + 1] = v2.y;
                 }
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-                    for (int j = 0; j < kPer; ++j) acc[j] += x[k][j] * c[k];
             }
         };
+        auto add = [&](int from, auto factor_of) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const float c = factor_of(min(from + k * step, parts - 1));
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) acc[j] += x[k][j] * c;
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
+        load(first);
         const size_t q_row = (size_t)b * p.d.n_q_heads + grp * rows + row;
         if (one_warp) {
-            if (!there) continue;
             const float2 ml = lane < parts ? p.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
             float m = ml.x;
 #pragma unroll
@@ -518,11 +584,16 @@ __global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(const DecodePa
             float l = ml.y * c;
 #pragma unroll
             for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-            sum_parts(0, 1, [&](int i) { return __shfl_sync(~0u, c, i); });
+            auto factor_of = [&](int i) { return __shfl_sync(~0u, c, i); };
+            add(0, factor_of);
+            for (int i = kBatch; i < parts; i += kBatch) {
+                load(i);
+                add(i, factor_of);
+            }
             const bool none = m == -INFINITY;  // no key at all
             const float inv = none ? 0.f : 1.f / l;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) store_out(p.d.out, q_row * D + j * 32 + lane, acc[j] * inv, p.d.out_dtype);
+            for (int j = 0; j < kPer; ++j) store_out(p.d.out, q_row * D + lane * kPer + j, acc[j] * inv, p.d.out_dtype);
             if (lane == 0) {
                 const float e = none ? -INFINITY : m + log2f(l);
                 p.lse2[q_row] = e;
@@ -530,7 +601,6 @@ __global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(const DecodePa
             }
             continue;
         }
-        if (!there) continue;
         float m = -INFINITY;
         float2 ml[kRounds];
 #pragma unroll
@@ -559,9 +629,14 @@ __global__ void __launch_bounds__(kJoinThreads) batch_join_kernel(const DecodePa
         for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
         if (lane == 0) sh_ml[warp].y = l;
         __syncthreads();
-        sum_parts(warp, kJoinWarps, [&](int i) { return factor[i]; });
+        auto factor_of = [&](int i) { return factor[i]; };
+        add(first, factor_of);
+        for (int i = first + step * kBatch; i < parts; i += step * kBatch) {
+            load(i);
+            add(i, factor_of);
+        }
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) sh_acc[warp][j * 32 + lane] = acc[j];
+        for (int j = 0; j < kPer; ++j) sh_acc[warp][lane * kPer + j] = acc[j];
         __syncthreads();
         l = 0.f;
 #pragma unroll
@@ -590,12 +665,15 @@ constexpr int kTotalsThreads = 256;
 __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const DecodeParams p) {
     extern __shared__ int chunks[];
     __shared__ int warp_sums[32];
-    pdl_wait();
-    pdl_trigger();
     const int G = p.group, hkv = p.v.hkv;
     constexpr int kPages = kTotalsThreads / kPageSlots;
-    scan_counts(p.v.batch, chunks, warp_sums,
-                [&](int b) { return (p.base[b + 1] - p.base[b] + kPages - 1) / kPages; });
+    // Chunks before each sequence, and units.
+    int* base = chunks + p.v.batch + 1;
+    scan_counts(p.v.batch, chunks, warp_sums, [&](int b) { return (units_of(p, b) + kPages - 1) / kPages; });
+    __syncthreads();
+    scan_counts(p.v.batch, base, warp_sums, [&](int b) { return units_of(p, b); });
+    pdl_wait();
+    pdl_trigger();
     const int64_t all = (int64_t)chunks[p.v.batch] * hkv;
     for (int64_t c = blockIdx.x; c < all; c += gridDim.x) {
         const int at = (int)(c / hkv), h = (int)(c - (int64_t)at * hkv);
@@ -603,10 +681,9 @@ __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const Deco
         const int t = (at - chunks[b]) * kTotalsThreads + threadIdx.x;
         const int n = attended(p.v, p.d, b, false);
         if (t >= n) continue;
-        const int base = p.base[b], count = p.base[b + 1] - base;
         const size_t place = ((size_t)b * hkv + h) * p.d.weights_stride + t;
         const float old = p.d.weights_in && t < p.v.lens[b] ? p.d.decay * p.d.weights_in[place] : 0.f;
-        const float* s = p.scores + (((size_t)base * hkv + (size_t)h * count) * kPageSlots + t) * G;
+        const float* s = p.scores + (((size_t)base[b] * hkv + (size_t)h * (base[b + 1] - base[b])) * kPageSlots + t) * G;
         const float* e = p.lse2 + (size_t)b * p.d.n_q_heads + h * G;
         float sum = 0.f;
         for (int g = 0; g < G; ++g) sum += exp2_of(s[g] - e[g]);
@@ -642,7 +719,7 @@ cudaError_t for_kernel(bool f16, int dim, bool two, F f) {
 size_t round16(size_t x) { return (x + 15) / 16 * 16; }
 
 struct DecodeSpace {
-    size_t acc, ml, lse2, base, scores, all;
+    size_t acc, ml, lse2, scores, all;
 };
 DecodeSpace decode_space(const BatchView& v, const BatchSplit& s, int n_q_heads, bool totals) {
     const size_t rows = (size_t)2 * s.workers * s.heads * (n_q_heads / v.hkv);
@@ -650,8 +727,7 @@ DecodeSpace decode_space(const BatchView& v, const BatchSplit& s, int n_q_heads,
     o.acc = 0;
     o.ml = o.acc + round16(rows * v.dim * sizeof(float));
     o.lse2 = o.ml + round16(rows * sizeof(float2));
-    o.base = o.lse2 + round16((size_t)v.batch * n_q_heads * sizeof(float));
-    o.scores = o.base + round16((size_t)(v.batch + 1) * sizeof(int32_t));
+    o.scores = o.lse2 + round16((size_t)v.batch * n_q_heads * sizeof(float));
     o.all = o.scores + (totals ? (size_t)v.batch * v.table_pages * kPageSlots * n_q_heads * sizeof(float) : 0);
     return o;
 }
@@ -698,7 +774,6 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
     p.part_acc = reinterpret_cast<float*>(w + o.acc);
     p.part_ml = reinterpret_cast<float2*>(w + o.ml);
     p.lse2 = reinterpret_cast<float*>(w + o.lse2);
-    p.base = reinterpret_cast<int32_t*>(w + o.base);
     p.scores = d.weights_out ? reinterpret_cast<float*>(w + o.scores) : nullptr;
     cudaError_t e = for_kernel(v.f16, v.dim, p.group > 8, [&](auto* k) {
         return launch_dependent(k, dim3(p.s.grid), dim3(p.s.warps * 32), smem_bytes(v.batch), stream, p);
@@ -708,12 +783,13 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
     // starting before the appended rows are in their pages.
     const int64_t items = (int64_t)v.batch * p.s.groups * p.s.heads * p.group;
     const dim3 grid((unsigned)std::min<int64_t>(items, (int64_t)v.sms * 8));
-    e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinThreads), 0, stream, p)
-        : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinThreads), 0, stream, p)
-                       : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinThreads), 0, stream, p);
+    const size_t base_bytes = sizeof(int) * (size_t)(v.batch + 1);
+    e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinThreads), base_bytes, stream, p)
+        : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinThreads), base_bytes, stream, p)
+                       : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinThreads), base_bytes, stream, p);
     if (e != cudaSuccess || !d.weights_out) return e;
     return launch_dependent(batch_totals_kernel, dim3(v.sms * 8), dim3(kTotalsThreads),
-                            sizeof(int) * (size_t)(v.batch + 1), stream, p);
+                            sizeof(int) * (size_t)(2 * v.batch + 2), stream, p);
 }
 
 }  // namespace gkv
