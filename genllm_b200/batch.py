@@ -37,6 +37,12 @@ def _invalid(message: str) -> GkvError:
     return GkvError(_lib.GKV_ERR_INVALID, message)
 
 
+def _current_stream(device: int) -> int:
+    """The current stream's handle (without a Stream object, where torch offers that)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def _expect(t: torch.Tensor, what: str, device: torch.device, dtype, shape, contiguous: bool = True) -> torch.Tensor:
     """t as a tensor of this device, type and shape (None: any extent)."""
     if not isinstance(t, torch.Tensor):
@@ -106,8 +112,8 @@ class _Bound:
 
     def __init__(self, cache: PagedBatch):
         self.cache = cache
-        self._home = torch.cuda.current_stream(cache.device)
-        self._home_handle = self._home.cuda_stream
+        self._device = cache.device.index
+        self._home = _current_stream(self._device)
         self._keep = [cache.k_pool, cache.v_pool, cache.table, cache.lens]
 
     def _hold(self, *tensors):
@@ -118,17 +124,21 @@ class _Bound:
         self._hold(t)
         return t
 
-    def _enqueue(self, stream) -> None:
-        raise NotImplementedError
+    def _bind(self, fn, *args, result):
+        self._fn, self._args, self._result = fn, args, result
 
-    def _run(self, stream) -> None:
-        s = stream if stream is not None else torch.cuda.current_stream(self.cache.device)
-        handle = s.cuda_stream
-        if stream is not None or handle != self._home_handle:
+    def run(self, stream=None) -> torch.Tensor:
+        """Enqueue on `stream` (default: the current one); the tensor it fills."""
+        handle = _current_stream(self._device) if stream is None else stream.cuda_stream
+        if stream is not None or handle != self._home:
             # Memory freed while this work is pending must not be handed out again on its own stream.
+            s = stream if stream is not None else torch.cuda.current_stream(self._device)
             for t in self._keep:
                 t.record_stream(s)
-        self._enqueue(handle)
+        status = self._fn(*self._args, handle)
+        if status:
+            check(status)
+        return self._result
 
 
 class BatchDecode(_Bound):
@@ -190,14 +200,7 @@ class BatchDecode(_Bound):
             float(scale) if scale is not None else float(d) ** -0.5, float(decay), space.data_ptr(), space.numel())
         self._hold(q, k_new, v_new, out, lse, pages, weights, weights_out)
         self.out, self.lse, self.weights_out = out, lse, weights_out
-        self._fn, self._a, self._b = lib().gkv_batch_decode, C.byref(cache.desc), C.byref(self.args)
-
-    def _enqueue(self, stream) -> None:
-        check(self._fn(self._a, self._b, stream))
-
-    def run(self, stream=None) -> torch.Tensor:
-        self._run(stream)
-        return self.out
+        self._bind(lib().gkv_batch_decode, C.byref(cache.desc), C.byref(self.args), result=out)
 
 
 class PageBounds(_Bound):
@@ -214,16 +217,8 @@ class PageBounds(_Bound):
             _expect(start, "start", cache.device, torch.int32, (cache.batch,))
         self._hold(bounds, start)
         self.bounds = bounds
-        self._fn, self._a = lib().gkv_batch_page_bounds, C.byref(cache.desc)
-        self._start = start.data_ptr() if start is not None else None
-        self._extra, self._to = int(extra), bounds.data_ptr()
-
-    def _enqueue(self, stream) -> None:
-        check(self._fn(self._a, self._start, self._extra, self._to, stream))
-
-    def run(self, stream=None) -> torch.Tensor:
-        self._run(stream)
-        return self.bounds
+        self._bind(lib().gkv_batch_page_bounds, C.byref(cache.desc), start.data_ptr() if start is not None else None,
+                   int(extra), bounds.data_ptr(), result=bounds)
 
 
 class PageSelect(_Bound):
@@ -253,14 +248,7 @@ class PageSelect(_Bound):
                                          space.data_ptr(), space.numel())
         self._hold(q, bounds, pages)
         self.pages = pages
-        self._fn, self._a, self._b = lib().gkv_batch_select_pages, C.byref(cache.desc), C.byref(self.args)
-
-    def _enqueue(self, stream) -> None:
-        check(self._fn(self._a, self._b, stream))
-
-    def run(self, stream=None) -> torch.Tensor:
-        self._run(stream)
-        return self.pages
+        self._bind(lib().gkv_batch_select_pages, C.byref(cache.desc), C.byref(self.args), result=pages)
 
 
 class CacheEvict(_Bound):
@@ -309,14 +297,7 @@ class CacheEvict(_Bound):
                                         shape[2], int(keep), int(recent), space.data_ptr(), space.numel())
         self._hold(weights, weights_out, positions, positions_out, seen, tracked, lens_out)
         self.lens_out, self.weights_out, self.positions_out = lens_out, weights_out, positions_out
-        self._fn, self._a, self._b = lib().gkv_batch_evict, C.byref(cache.desc), C.byref(self.args)
-
-    def _enqueue(self, stream) -> None:
-        check(self._fn(self._a, self._b, stream))
-
-    def run(self, stream=None) -> torch.Tensor:
-        self._run(stream)
-        return self.lens_out
+        self._bind(lib().gkv_batch_evict, C.byref(cache.desc), C.byref(self.args), result=lens_out)
 
 
 def batch_decode(cache: PagedBatch, q, k_new=None, v_new=None, *, stream=None, **options) -> torch.Tensor:

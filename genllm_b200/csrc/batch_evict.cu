@@ -47,10 +47,11 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 
 // One cluster per (sequence, head), one slice of its slots per CTA; a warp
 // takes a run of its slice, so ranks in slot order are ballots and prefix sums.
+template <bool LONE>
 __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const EvictParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ uint32_t slice_keys[];
-    __shared__ CutShared<uint32_t, kPlanThreads> cut_shared;
+    __shared__ CutShared<uint32_t, kPlanThreads, LONE> cut_shared;
     __shared__ int slots[kPlanWarps];
     __shared__ int2 rank_slots[2][kMaxCluster];
     pdl_trigger();
@@ -58,7 +59,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     cg::cluster_group cluster = cg::this_cluster();
     const BatchView& v = p.v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int ranks = LONE ? 1 : cluster.num_blocks(), rank = LONE ? 0 : cluster.block_rank();
     const int bh = blockIdx.x / ranks, b = bh / v.hkv;
     const int len = v.lens[b];
     const int cap = v.table_pages * kPageSlots;
@@ -107,8 +108,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
         }
     }
     __syncthreads();
-    uint32_t top = 0;
-    const Cut<uint32_t> cut = cluster_cut<uint32_t, kPlanThreads>(keys, m, left, kRecent, &top, cut_shared);
+    const Cut<uint32_t> cut = row_cut<uint32_t, kPlanThreads, LONE>(keys, m, left, kRecent, cut_shared);
 
     // A warp's run of the slice.
     const int run = ((m + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
         mine = __reduce_add_sync(~0u, mine);
         int all;
         equal = warps_before<kPlanThreads>(mine, slots, &all);
-        equal += cluster_before(make_int2(all, 0), rank_slots[0]).x;
+        equal += row_before<LONE>(make_int2(all, 0), rank_slots[0]).x;
     }
     auto kept_of = [&](int i, int* seen_equal) {
         const uint32_t k = i < i1 ? keys[i] : 0;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     int hole_all, source_all;
     int hole_at = warps_before<kPlanThreads>(holes, slots, &hole_all);
     int source_at = warps_before<kPlanThreads>(sources, slots, &source_all);
-    const int2 before = cluster_before(make_int2(hole_all, source_all), rank_slots[1]);
+    const int2 before = row_before<LONE>(make_int2(hole_all, source_all), rank_slots[1]);
     hole_at += before.x;
     source_at += before.y;
     if (rank == ranks - 1 && tid == kPlanThreads - 1) {
@@ -262,8 +262,11 @@ EvictSpace evict_space(const BatchView& v) {
 size_t evict_bytes(const BatchView& v) { return evict_space(v).all; }
 
 cudaError_t configure_evict() {
-    return cudaFuncSetAttribute(evict_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kMaxSlice * (int)sizeof(uint32_t));
+    const int most = kMaxSlice * (int)sizeof(uint32_t);
+    const cudaError_t e = cudaFuncSetAttribute(evict_plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return e != cudaSuccess
+               ? e
+               : cudaFuncSetAttribute(evict_plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
 }
 
 cudaError_t launch_evict(const BatchView& v, const EvictLaunch& e, cudaStream_t stream) {
@@ -277,7 +280,7 @@ cudaError_t launch_evict(const BatchView& v, const EvictLaunch& e, cudaStream_t 
                   reinterpret_cast<Move*>(w + s.moves),
                   s.spill ? reinterpret_cast<uint32_t*>(w + s.keys) : nullptr};
     const size_t slice = ((cap + s.cluster - 1) / s.cluster + 31) / 32 * 32;
-    cudaError_t err = launch_cluster(evict_plan_kernel, (unsigned)heads, s.cluster, kPlanThreads,
+    cudaError_t err = launch_cluster(s.cluster == 1 ? evict_plan_kernel<true> : evict_plan_kernel<false>, (unsigned)heads, s.cluster, kPlanThreads,
                                      s.spill ? 0 : slice * sizeof(uint32_t), stream, p);
     if (err != cudaSuccess) return err;
     // About eight CTAs per SM over all heads.

@@ -119,8 +119,11 @@ struct SelectParams {
     BatchView v;
     SelectLaunch s;
     int32_t group;
+    int32_t heads, groups, lanes, workers;  // of the score kernel, as in the decode kernel's split
+    uint32_t* approx;  // [batch][hkv][table_pages]
+    uint32_t* tops;    // [batch][hkv][tiles of 16 pages] largest |bound|, as bits
     uint64_t* exact;   // [batch][hkv][table_pages], where many pages lie at the cut
-    uint32_t* approx;  // [batch][hkv][table_pages] where a slice does not fit in shared memory; else null
+    bool spill;        // a slice of keys does not fit in shared memory
 };
 
 // Scores as integers of the same order, above 0; a page taken in any case
@@ -140,9 +143,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key >> 31 ? key & 0x7FFFFFFFu : ~key);
 }
 
-constexpr int kSelectThreads = 256;
-constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kMaxSlice = 32768;  // keys of a CTA in shared memory: 128 KB
+constexpr int kScoreWarps = 8;
+constexpr int kPickThreads = 512;
+constexpr int kPickWarps = kPickThreads / 32;
+constexpr int kMaxSlice = 16384;  // keys of a CTA in shared memory: 64 KB
 constexpr int kMaxClose = 64;     // pages at the cut that are ranked in shared memory
 
 // E of the tensor cores' score, relative to max |bound| * sum |q|: each of the
@@ -186,139 +190,211 @@ __device__ uint64_t exact_key(const SelectParams& p, int b, int h, int page) {
     return nan ? kNaN : key_of(best);
 }
 
-// One cluster per (sequence, head), a slice of its pages per CTA.
+// Scores on the tensor cores, sixteen pages a step of a warp: the tiles of all
+// sequences form one line, cut equally between the workers (one warp per kv
+// head of a group), so that ragged batches load every SM alike. Step k of the
+// product takes two pairs of dims of the 16-byte chunk that a lane loads of a
+// page's row, so rows go from memory to the A fragment as they are. Bound: HBM.
 template <bool F16, int D, int NT>
-__global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const SelectParams p) {
-    namespace cg = cooperative_groups;
+__global__ void __launch_bounds__(kScoreWarps * 32, NT == 1 && D <= 128 ? 2 : 1) page_score_kernel(const SelectParams p) {
     constexpr int kLoads = D / 32;  // 16-byte chunks of a lane's row, of either bound
+    extern __shared__ int base[];   // tiles before each sequence
+    __shared__ int warp_sums[32];
+    pdl_wait();
+    pdl_trigger();
+    const BatchView& v = p.v;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto pages_in = [&](int b, bool flag) { return pages_of(tokens_of(v, b, p.s.extra, flag)); };
+    scan_counts(v.batch, base, warp_sums, [&](int b) {
+        const int pages = pages_in(b, blockIdx.x == 0);
+        return pages <= p.s.n_pages ? 0 : (pages + 15) / 16;  // fewer pages than places: all are taken
+    });
+    if (warp >= p.lanes * p.heads) return;
+    const int total = base[v.batch] * p.groups, per = max(1, (total + p.workers - 1) / p.workers);
+    const int worker = blockIdx.x * p.lanes + warp / p.heads, head_in = warp % p.heads;
+    const int u0 = (int)min((int64_t)total, (int64_t)worker * per), u1 = min(total, u0 + per);
+    const int quarter = lane & 3;
+    const int max_tiles = (v.table_pages + 15) / 16;
+
+    for (int u = u0; u < u1;) {
+        const int b = owner(base, v.batch, p.groups, u);
+        const int tiles = base[b + 1] - base[b], grp = (u - base[b] * p.groups) / tiles;
+        const int seg0 = base[b] * p.groups + grp * tiles, end = min(u1, seg0 + tiles);
+        const int h = grp * p.heads + head_in;
+        if (h >= v.hkv) {
+            u = end;
+            continue;
+        }
+        // max(q, 0) for hi, min(q, 0) for lo, as B fragments.
+        uint2 f[2][kLoads][2][NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int g = nt * 8 + (lane >> 2);
+            const uint16_t* row = p.s.q + b * p.s.q_stride_batch + (int64_t)(h * p.group + g) * p.s.q_stride_head + quarter * 8;
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k) {
+                const uint4 x = g < p.group ? *reinterpret_cast<const uint4*>(row + k * 32) : make_uint4(0, 0, 0, 0);
+                auto split = [](uint32_t w, uint32_t& pos, uint32_t& neg) {
+                    const uint32_t mask = ((w >> 15 & 1) * 0xFFFFu) | ((w >> 31) * 0xFFFF0000u);
+                    pos = w & ~mask;
+                    neg = w & mask;
+                };
+                split(x.x, f[0][k][0][nt].x, f[1][k][0][nt].x);
+                split(x.y, f[0][k][0][nt].y, f[1][k][0][nt].y);
+                split(x.z, f[0][k][1][nt].x, f[1][k][1][nt].x);
+                split(x.w, f[0][k][1][nt].y, f[1][k][1][nt].y);
+            }
+        }
+        const int pages = pages_in(b, false);
+        const int2* table = v.table + b * v.table_stride;
+        uint32_t* keys = p.approx + ((size_t)b * v.hkv + h) * v.table_pages;
+        uint32_t* tops = p.tops + ((size_t)b * v.hkv + h) * max_tiles;
+        // This lane's rows are pages lane / 4 and lane / 4 + 8 of a tile.
+        int next[2];
+        auto fetch = [&](int tile) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) next[r] = table[min(tile * 16 + r * 8 + (lane >> 2), pages - 1)].x;
+        };
+        fetch(u - seg0);
+        for (; u < end; ++u) {
+            const int tile = u - seg0;
+            bool bad[2];
+            const uint4* row[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                bad[r] = next[r] < 0 || next[r] >= v.pool_pages;
+                row[r] = reinterpret_cast<const uint4*>(p.s.bounds + ((size_t)(bad[r] ? 0 : next[r]) * v.hkv + h) * 2 * D) + quarter;
+            }
+            uint32_t top = 0;
+            float c[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+            constexpr int kHalves = D == 256 ? 2 : 1;  // bounds in flight: both, or one after the other
+#pragma unroll
+            for (int part = 0; part < kHalves; ++part) {
+                constexpr int kTogether = 2 / kHalves;
+                uint4 x[kTogether][2][kLoads];
+#pragma unroll
+                for (int w = 0; w < kTogether; ++w)
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) x[w][r][k] = __ldcs(row[r] + k * 4 + (part + w == 0 ? D / 8 : 0));
+                if (part == 0) fetch(min(tile + 1, tiles - 1));
+#pragma unroll
+                for (int w = 0; w < kTogether; ++w) {
+                    const int low = part + w;
+#pragma unroll
+                    for (int k = 0; k < kLoads; ++k) {
+                        const uint32_t a[2][4] = {{x[w][0][k].x, x[w][1][k].x, x[w][0][k].y, x[w][1][k].y},
+                                                  {x[w][0][k].z, x[w][1][k].z, x[w][0][k].w, x[w][1][k].w}};
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            top = __vmaxu2(top, __vmaxu2(a[half][0] & 0x7FFF7FFFu, a[half][1] & 0x7FFF7FFFu));
+                            top = __vmaxu2(top, __vmaxu2(a[half][2] & 0x7FFF7FFFu, a[half][3] & 0x7FFF7FFFu));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma16816<F16>(c[nt], a[half], f[low][k][half][nt].x, f[low][k][half][nt].y);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float best = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (nt * 8 + quarter * 2 + j < p.group) best = fmaxf(best, c[nt][r * 2 + j]);
+                best = fmaxf(best, __shfl_xor_sync(~0u, best, 1));
+                best = fmaxf(best, __shfl_xor_sync(~0u, best, 2));
+                const int lp = tile * 16 + r * 8 + (lane >> 2);
+                if (quarter == 0 && lp < pages) {
+                    const bool taken = lp < p.s.n_first || lp >= pages - p.s.n_last;
+                    if (bad[r] && !taken) atomicOr(v.err, kErrBadPage);
+                    keys[lp] = taken ? kTaken32 : bad[r] ? 1u : key32_of(best);
+                }
+            }
+            top = __reduce_max_sync(~0u, max(top & 0xFFFFu, top >> 16));
+            if (lane == 0) tops[tile] = top;
+        }
+    }
+}
+
+// The taken pages of each (sequence, head) in rising order, one CTA or cluster
+// a row. Bound: latency (a chain of barriers over a few kilobytes).
+template <bool F16, int D, bool LONE>
+__global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectParams p) {
     struct Close {
         uint64_t key;
         int page;
     };
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ CutShared<uint32_t, kSelectThreads> cut_shared;
-    __shared__ CutShared<uint64_t, kSelectThreads> exact_shared;
+    extern __shared__ uint32_t slice_keys[];
+    __shared__ union {
+        CutShared<uint32_t, kPickThreads, LONE> approx;
+        CutShared<uint64_t, kPickThreads, LONE> exact;
+    } cut_shared;
     __shared__ Close close[kMaxClose];
     __shared__ int close_page[kMaxClose];
-    __shared__ int slots[kSelectWarps];
+    __shared__ int slots[kPickWarps];
     __shared__ int2 rank_slots[3][kMaxCluster];
-    __shared__ uint32_t warp_top[kSelectWarps];
+    __shared__ uint32_t warp_top[kPickWarps];
     __shared__ float head_sum[kMaxBatchGroup];
-    pdl_wait();
-    pdl_trigger();
-    cg::cluster_group cluster = cg::this_cluster();
     const BatchView& v = p.v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int ranks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int ranks = LONE ? 1 : cooperative_groups::this_cluster().num_blocks();
+    const int rank = LONE ? 0 : cooperative_groups::this_cluster().block_rank();
     const int bh = blockIdx.x / ranks, b = bh / v.hkv, h = bh % v.hkv;
-    if (v.lens[b] < 0) return;  // the whole cluster
-    const int pages = pages_of(tokens_of(v, b, p.s.extra, rank == 0 && tid == 0));
-    int32_t* to = p.s.pages + (size_t)bh * p.s.n_pages;
-    const int take = min(p.s.n_pages, pages);
-    for (int i = take + rank * kSelectThreads + tid; i < p.s.n_pages; i += ranks * kSelectThreads) to[i] = -1;
-    if (pages <= p.s.n_pages) {
-        for (int i = rank * kSelectThreads + tid; i < pages; i += ranks * kSelectThreads) to[i] = i;
-        return;  // the whole cluster
-    }
-    const int slice = ((pages + ranks - 1) / ranks + 31) / 32 * 32;
-    const int p0 = min(pages, rank * slice), m = min(pages - p0, slice);
-    const int2* table = v.table + b * v.table_stride;
-
-    // Queries as B fragments: step k of the product takes two pairs of dims of
-    // the 16-byte chunk that a lane loads of a page's row, so rows go from
-    // memory to the A fragment as they are. First max(q, 0) (for hi), then min.
-    uint2* frag = reinterpret_cast<uint2*>(smem);  // [2][kLoads][2][NT][32]
-    constexpr int kFrags = 2 * kLoads * 2 * NT * 32;
-    for (int i = tid; i < kFrags; i += kSelectThreads) {
-        const int l = i & 31, nt = i / 32 % NT, half = i / (32 * NT) % 2, k = i / (64 * NT) % kLoads, low = i / (64 * NT * kLoads);
-        const int g = nt * 8 + (l >> 2);
-        uint2 x = make_uint2(0, 0);
-        if (g < p.group) {
-            const uint16_t* row = p.s.q + b * p.s.q_stride_batch + (int64_t)(h * p.group + g) * p.s.q_stride_head;
-            x = *reinterpret_cast<const uint2*>(row + (k * 4 + (l & 3)) * 8 + half * 4);
-            auto part = [&](uint32_t w) {
-                const uint32_t neg = ((w >> 15 & 1) * 0xFFFFu) | ((w >> 31) * 0xFFFF0000u);
-                return w & (low ? neg : ~neg);
-            };
-            x.x = part(x.x);
-            x.y = part(x.y);
-        }
-        frag[i] = x;
-    }
-    for (int g = warp; g < p.group; g += kSelectWarps) {
+    // Ahead of the wait: what the score kernel's own predecessors wrote (it lets
+    // this one start once they are done), past L1.
+    const int len = __ldcg(v.lens + b), cap = v.table_pages * kPageSlots;
+    const int pages = len < 0 ? 0 : pages_of(min(len, cap - p.s.extra) + p.s.extra);
+    for (int g = warp; g < p.group; g += kPickWarps) {
         float sum = 0.f;
-        const uint16_t* row = p.s.q + b * p.s.q_stride_batch + (int64_t)(h * p.group + g) * p.s.q_stride_head;
-        for (int d = lane; d < D; d += 32) sum += fabsf(floats_of<F16>(row[d]).x);
+        const uint32_t* row = reinterpret_cast<const uint32_t*>(p.s.q + b * p.s.q_stride_batch +
+                                                                (int64_t)(h * p.group + g) * p.s.q_stride_head);
+        for (int d = lane; d < D / 2; d += 32) {
+            const float2 x = floats_of<F16>(__ldcg(row + d));
+            sum += fabsf(x.x) + fabsf(x.y);
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
         if (lane == 0) head_sum[g] = sum;
     }
-    uint32_t* keys = p.approx ? p.approx + (size_t)bh * v.table_pages + p0
-                              : reinterpret_cast<uint32_t*>(smem + kFrags * sizeof(uint2));
-    __syncthreads();
-
-    // Sixteen pages a warp: this lane's rows are pages lane / 4 and lane / 4 + 8.
-    const int quarter = lane & 3;
-    uint32_t top = 0;  // largest |bound|, as bits
-    for (int i0 = warp * 16; i0 < m; i0 += kSelectWarps * 16) {
-        int page[2];
-        bool bad[2];
-        const uint4* row[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            page[r] = table[p0 + min(i0 + r * 8 + (lane >> 2), m - 1)].x;
-            bad[r] = page[r] < 0 || page[r] >= v.pool_pages;
-            row[r] = reinterpret_cast<const uint4*>(p.s.bounds + ((size_t)(bad[r] ? 0 : page[r]) * v.hkv + h) * 2 * D) + quarter;
-        }
-        float c[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-#pragma unroll
-        for (int low = 0; low < 2; ++low) {
-            uint4 x[2][kLoads];
-#pragma unroll
-            for (int k = 0; k < kLoads; ++k)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) x[r][k] = row[r][k * 4 + (low ? 0 : D / 8)];
-#pragma unroll
-            for (int k = 0; k < kLoads; ++k) {
-                const uint32_t a[2][4] = {{x[0][k].x, x[1][k].x, x[0][k].y, x[1][k].y},
-                                          {x[0][k].z, x[1][k].z, x[0][k].w, x[1][k].w}};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    top = __vmaxu2(top, __vmaxu2(a[half][0] & 0x7FFF7FFFu, a[half][1] & 0x7FFF7FFFu));
-                    top = __vmaxu2(top, __vmaxu2(a[half][2] & 0x7FFF7FFFu, a[half][3] & 0x7FFF7FFFu));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const uint2 f = frag[(((low * kLoads + k) * 2 + half) * NT + nt) * 32 + lane];
-                        mma16816<F16>(c[nt], a[half], f.x, f.y);
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float best = -INFINITY;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (nt * 8 + quarter * 2 + j < p.group) best = fmaxf(best, c[nt][r * 2 + j]);
-            best = fmaxf(best, __shfl_xor_sync(~0u, best, 1));
-            best = fmaxf(best, __shfl_xor_sync(~0u, best, 2));
-            const int i = i0 + r * 8 + (lane >> 2), lp = p0 + i;
-            if (quarter == 0 && i < m) {
-                const bool taken = lp < p.s.n_first || lp >= pages - p.s.n_last;
-                if (bad[r] && !taken) atomicOr(v.err, kErrBadPage);
-                keys[i] = taken ? kTaken32 : bad[r] ? 1u : key32_of(best);
-            }
-        }
+    pdl_wait();
+    pdl_trigger();
+    if (len < 0) return;  // the whole row
+    int32_t* to = p.s.pages + (size_t)bh * p.s.n_pages;
+    const int take = min(p.s.n_pages, pages);
+    for (int i = take + rank * kPickThreads + tid; i < p.s.n_pages; i += ranks * kPickThreads) to[i] = -1;
+    if (pages <= p.s.n_pages) {
+        for (int i = rank * kPickThreads + tid; i < pages; i += ranks * kPickThreads) to[i] = i;
+        return;  // the whole row
     }
-    top = __reduce_max_sync(~0u, max(top & 0xFFFFu, top >> 16));
+    const int slice = ((pages + ranks - 1) / ranks + 31) / 32 * 32;
+    const int p0 = min(pages, rank * slice), m = min(pages - p0, slice);
+    const int2* table = v.table + b * v.table_stride;
+    uint32_t* keys = p.approx + (size_t)bh * v.table_pages + p0;
+    if (!p.spill) {
+        for (int i = tid; i < m; i += 8 * kPickThreads) {
+            uint32_t x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = keys[min(i + j * kPickThreads, m - 1)];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j * kPickThreads < m) slice_keys[i + j * kPickThreads] = x[j];
+        }
+        keys = slice_keys;
+    }
+    // Every CTA looks at all tiles' largest bounds.
+    const int max_tiles = (v.table_pages + 15) / 16;
+    uint32_t top = 0;
+    for (int i = tid; i < (pages + 15) / 16; i += kPickThreads) top = max(top, p.tops[(size_t)bh * max_tiles + i]);
+    top = __reduce_max_sync(~0u, top);
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    top = __reduce_max_sync(~0u, lane < kSelectWarps ? warp_top[lane] : 0u);
-    const Cut<uint32_t> cut = cluster_cut<uint32_t, kSelectThreads>(keys, m, take, kTaken32, &top, cut_shared);
+    top = __reduce_max_sync(~0u, lane < kPickWarps ? warp_top[lane] : 0u);
+    const Cut<uint32_t> cut = row_cut<uint32_t, kPickThreads, LONE>(keys, m, take, kTaken32, cut_shared.approx);
 
     // Pages above `in` are taken and pages below `out` are not, whatever the
     // error; without a finite one (infinities, NaN) every page is in question.
@@ -337,7 +413,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
         if (cut.lo > kKeyMinusInf) out = key32_of(low - 2.f * error - fabsf(low) * 0x1p-22f);
     }
     // A warp's run of the slice, in page order.
-    const int run = ((m + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+    const int run = ((m + kPickWarps - 1) / kPickWarps + 31) / 32 * 32;
     const int i0 = min(m, warp * run), i1 = min(m, i0 + run);
     const uint32_t below = (1u << lane) - 1;
     int above = 0, at_cut = 0, above_all, cut_all;
@@ -346,17 +422,17 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
         above += __popc(__ballot_sync(~0u, k > in));
         at_cut += __popc(__ballot_sync(~0u, k >= out && k <= in));
     }
-    int above_at = warps_before<kSelectThreads>(above, slots, &above_all);
-    int cut_at = warps_before<kSelectThreads>(at_cut, slots, &cut_all);
-    const int2 before = cluster_before(make_int2(above_all, cut_all), rank_slots[0]);
+    int above_at = warps_before<kPickThreads>(above, slots, &above_all);
+    int cut_at = warps_before<kPickThreads>(at_cut, slots, &cut_all);
+    const int2 before = row_before<LONE>(make_int2(above_all, cut_all), rank_slots[0]);
     above_at += before.x;
     cut_at += before.y;
     // The row's totals: every rank's pair is in the slots.
     const int2 each = lane < ranks ? rank_slots[0][lane] : make_int2(0, 0);
-    const int row_above = __reduce_add_sync(~0u, each.x), row_cut = __reduce_add_sync(~0u, each.y);
+    const int row_above = __reduce_add_sync(~0u, each.x), row_close = __reduce_add_sync(~0u, each.y);
     const int want = take - row_above;
 
-    if (want == row_cut || want <= 0) {
+    if (want == row_close || want <= 0) {
         // Nothing at the cut is left out (or, with forced pages alone, taken).
         int place = above_at + (want > 0 ? cut_at : 0);
         const uint32_t least = want > 0 ? out : in + 1;
@@ -367,7 +443,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
         }
         return;
     }
-    if (row_cut <= kMaxClose) {
+    if (row_close <= kMaxClose) {
         // Every rank gets the exact scores of the few pages at the cut and ranks them itself.
         int at = cut_at;
         for (int i = i0; i < i1; i += 32) {
@@ -377,21 +453,21 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
             at += __popc(mask);
         }
         __syncthreads();
-        for (int i = before.y + warp; i < before.y + cut_all; i += kSelectWarps) {
+        for (int i = before.y + warp; i < before.y + cut_all; i += kPickWarps) {
             const int lp = close_page[i], page = table[lp].x;
             const uint64_t key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, b, h, page);
             if (lane < ranks) {
-                Close* remote = cluster.map_shared_rank(close, lane);
+                Close* remote = at_rank<LONE>(close, lane);
                 remote[i].key = key;
                 remote[i].page = lp;
             }
         }
-        cluster.sync();
+        row_sync<LONE>();
         // keys at the cut become 0 (left out) or kTaken32.
-        for (int i = tid; i < row_cut; i += kSelectThreads) {
+        for (int i = tid; i < row_close; i += kPickThreads) {
             const Close mine = close[i];
             int better = 0;
-            for (int j = 0; j < row_cut; ++j)
+            for (int j = 0; j < row_close; ++j)
                 better += close[j].key > mine.key || (close[j].key == mine.key && close[j].page < mine.page);
             close_page[i] = better < want;
             if (mine.page >= p0 && mine.page < p0 + m) keys[mine.page - p0] = better < want ? kTaken32 : 0;
@@ -418,14 +494,13 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
         if (lane == 0) exact[i] = key;
     }
     __syncthreads();
-    uint32_t unused = 0;
-    const Cut<uint64_t> fine = cluster_cut<uint64_t, kSelectThreads>(exact, m, take, kTaken, &unused, exact_shared);
+    const Cut<uint64_t> fine = row_cut<uint64_t, kPickThreads, LONE>(exact, m, take, kTaken, cut_shared.exact);
     int equal = 0;  // keys of the cut's range before this run
     if (fine.partial) {
         int mine = 0, all;
         for (int i = i0 + lane; i < i1; i += 32) mine += exact[i] >= fine.lo && exact[i] <= fine.hi;
-        equal = warps_before<kSelectThreads>(__reduce_add_sync(~0u, mine), slots, &all);
-        equal += cluster_before(make_int2(all, 0), rank_slots[1]).x;
+        equal = warps_before<kPickThreads>(__reduce_add_sync(~0u, mine), slots, &all);
+        equal += row_before<LONE>(make_int2(all, 0), rank_slots[1]).x;
     }
     auto kept_mask = [&](int i, int* seen_equal) {
         const uint64_t k = i < i1 ? exact[i] : 0;
@@ -440,8 +515,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2) page_select_kernel(const Se
     };
     int count = 0, at = equal, all;
     for (int i = i0; i < i1; i += 32) count += __popc(kept_mask(i + lane, &at));
-    int place = warps_before<kSelectThreads>(count, slots, &all);
-    place += cluster_before(make_int2(all, 0), rank_slots[2]).x;
+    int place = warps_before<kPickThreads>(count, slots, &all);
+    place += row_before<LONE>(make_int2(all, 0), rank_slots[2]).x;
     at = equal;
     for (int i = i0; i < i1; i += 32) {
         const uint32_t mask = kept_mask(i + lane, &at);
@@ -469,21 +544,22 @@ struct LaunchBounds {
 };
 struct SelectSpace {
     int cluster;
-    bool spill;  // approximate keys in the workspace
-    size_t slice, approx, all;
+    bool spill;
+    size_t slice, tops, all;
 };
 SelectSpace select_space(const BatchView& v) {
-    const size_t rows = (size_t)v.batch * v.hkv;
+    const size_t rows = (size_t)v.batch * v.hkv, pages = (size_t)v.table_pages;
     SelectSpace s;
-    s.cluster = cluster_for((int)rows, v.table_pages, v.sms, 128, kMaxSlice);
-    s.slice = (((size_t)v.table_pages + s.cluster - 1) / s.cluster + 31) / 32 * 32;
+    // A lone CTA while its slice fits: barriers of a cluster cost more than the keys it saves.
+    s.cluster = 1;
+    while (s.cluster < kMaxCluster && (pages + s.cluster - 1) / s.cluster > kMaxSlice) s.cluster *= 2;
+    s.slice = ((pages + s.cluster - 1) / s.cluster + 31) / 32 * 32;
     s.spill = s.slice > kMaxSlice;
-    s.approx = rows * v.table_pages * sizeof(uint64_t);
-    s.all = s.approx + (s.spill ? rows * v.table_pages * sizeof(uint32_t) : 0);
+    const size_t approx = rows * pages * sizeof(uint64_t);
+    s.tops = approx + rows * pages * sizeof(uint32_t);
+    s.all = s.tops + rows * ((pages + 15) / 16) * sizeof(uint32_t);
     return s;
 }
-
-size_t frag_bytes(int dim, int tiles) { return (size_t)2 * (dim / 32) * 2 * tiles * 32 * sizeof(uint2); }
 
 struct LaunchSelect {
     SelectParams p;
@@ -491,20 +567,27 @@ struct LaunchSelect {
     cudaStream_t stream;
     template <bool F16, int D>
     cudaError_t operator()() const {
-        const int tiles = p.group > 8 ? 2 : 1;
-        const size_t smem = frag_bytes(D, tiles) + (s.spill ? 0 : s.slice * sizeof(uint32_t));
-        return launch_cluster(tiles == 2 ? page_select_kernel<F16, D, 2> : page_select_kernel<F16, D, 1>,
-                              (unsigned)(p.v.batch * p.v.hkv), s.cluster, kSelectThreads, smem, stream, p);
+        const int ctas = D <= 128 && p.group <= 8 ? 2 : 1;  // of an SM
+        SelectParams q = p;
+        q.workers = p.v.sms * ctas * p.lanes;
+        const size_t base = sizeof(int) * (size_t)(p.v.batch + 1);
+        const dim3 grid(p.v.sms * ctas), block(kScoreWarps * 32);
+        cudaError_t e = p.group > 8 ? launch_dependent(page_score_kernel<F16, D, 2>, grid, block, base, stream, q)
+                                    : launch_dependent(page_score_kernel<F16, D, 1>, grid, block, base, stream, q);
+        if (e != cudaSuccess) return e;
+        return launch_cluster(s.cluster == 1 ? page_pick_kernel<F16, D, true> : page_pick_kernel<F16, D, false>,
+                              (unsigned)(p.v.batch * p.v.hkv), s.cluster, kPickThreads,
+                              s.spill ? 0 : s.slice * sizeof(uint32_t), stream, q);
     }
 };
 struct ConfigureSelect {
     template <bool F16, int D>
     cudaError_t operator()() const {
-        const int most = (int)(frag_bytes(D, 2) + kMaxSlice * sizeof(uint32_t));
-        cudaError_t e = cudaFuncSetAttribute(page_select_kernel<F16, D, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(page_select_kernel<F16, D, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        return e;
+        const int most = kMaxSlice * (int)sizeof(uint32_t);
+        const cudaError_t e = cudaFuncSetAttribute(page_pick_kernel<F16, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        return e != cudaSuccess ? e
+                                : cudaFuncSetAttribute(page_pick_kernel<F16, D, false>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     }
 };
 
@@ -532,8 +615,18 @@ cudaError_t configure_select() {
 cudaError_t launch_select_pages(const BatchView& v, const SelectLaunch& s, cudaStream_t stream) {
     const SelectSpace space = select_space(v);
     char* w = static_cast<char*>(s.workspace);
-    const SelectParams p{v, s, s.n_q_heads / v.hkv, reinterpret_cast<uint64_t*>(w),
-                         space.spill ? reinterpret_cast<uint32_t*>(w + space.approx) : nullptr};
+    SelectParams p;
+    p.v = v;
+    p.s = s;
+    p.group = s.n_q_heads / v.hkv;
+    p.heads = v.hkv < kScoreWarps ? v.hkv : kScoreWarps;
+    p.groups = (v.hkv + p.heads - 1) / p.heads;
+    p.lanes = kScoreWarps / p.heads;
+    p.workers = 0;
+    p.exact = reinterpret_cast<uint64_t*>(w);
+    p.approx = reinterpret_cast<uint32_t*>(w + (size_t)v.batch * v.hkv * v.table_pages * sizeof(uint64_t));
+    p.tops = reinterpret_cast<uint32_t*>(w + space.tops);
+    p.spill = space.spill;
     return by_type(v, LaunchSelect{p, space, stream});
 }
 

@@ -1,12 +1,13 @@
-// cut.cuh — the `want` largest of a row of integer keys, by a cluster of CTAs.
+// cut.cuh — the `target` largest of a row of integer keys, by one CTA or by a
+// cluster of them.
 //
 // Each CTA holds a slice of the row. Per pass the range [lo, hi] of the keys
-// that are still undecided is cut into at most 512 equal buckets, counted in
-// shared memory and summed over the cluster through distributed shared
-// memory; the bucket the cut falls into becomes the next range. Starting from
-// the keys' own smallest and largest values, a spread row is cut in one or
-// two or three passes, any row in ceil(bits / 9). 512 buckets and not 2048: a
-// CTA reads every rank's counts, and 2048 of them took longer than the pass
+// that are still undecided is cut into equal buckets, counted in shared memory
+// and summed over the cluster through distributed shared memory; the bucket
+// the cut falls into becomes the next range. Starting from the keys' own
+// smallest and largest values, a spread row is cut in one to three passes, any
+// row in ceil(bits / BITS). A lone CTA takes 2048 buckets; in a cluster 512, as
+// each CTA reads every rank's counts and 2048 of them took longer than the pass
 // they save.
 #pragma once
 #include <cooperative_groups.h>
@@ -23,38 +24,61 @@ struct Cut {
     bool partial;  // more keys in [lo, hi] than ties
 };
 
-constexpr int kCutBits = 9, kCutBins = 1 << kCutBits;
 constexpr int kMaxCluster = 8;
 
-template <typename K, int THREADS>
+// A row's barrier, and rank r's copy of a shared variable.
+template <bool LONE>
+__device__ __forceinline__ void row_sync() {
+    if (LONE) __syncthreads();
+    else cooperative_groups::this_cluster().sync();
+}
+template <bool LONE, typename T>
+__device__ __forceinline__ T* at_rank(T* p, int r) {
+    return LONE ? p : cooperative_groups::this_cluster().map_shared_rank(p, r);
+}
+
+template <typename K, int THREADS, bool LONE>
 struct CutShared {
-    int hist[2][kCutBins];
+    static constexpr int kBits = LONE ? 11 : 9, kBins = 1 << kBits;
+    int hist[2][kBins];
     K range[2];       // this CTA's smallest and largest undecided key
     int2 counts;      // how many keys it takes first, and how many others it has
-    uint32_t top;     // and its part of the row's `top`
     K warp_lo[THREADS / 32], warp_hi[THREADS / 32];
     int warp_sum[THREADS / 32], warp_rest[THREADS / 32];
-    int found[3];     // bucket, keys above it, keys in it
+    int found[2][3];  // bucket, keys above it, keys in it
 };
 
 __device__ __forceinline__ int bit_length(uint32_t x) { return 32 - __clz((int)x); }
 __device__ __forceinline__ int bit_length(uint64_t x) { return 64 - __clzll((long long)x); }
 
+template <typename K>
+__device__ __forceinline__ void range_reduce(K& lo, K& hi) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(~0u, lo, o));
+        hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+    }
+}
+template <>
+__device__ __forceinline__ void range_reduce<uint32_t>(uint32_t& lo, uint32_t& hi) {
+    lo = __reduce_min_sync(~0u, lo);
+    hi = __reduce_max_sync(~0u, hi);
+}
+
 // The largest `target` keys of the row. Keys of `skip` and above come before
-// all others, and among themselves by row order; the row holds at least
-// `target` keys that are not 0 (with fewer, all are taken); keys of 0 stand aside. *top: a value per CTA in, its maximum
-// over the row out. Every thread of the cluster calls it, after a
-// __syncthreads behind the writes of keys[0, n); it reads other CTAs' shared memory until
-// its return, so the caller passes a cluster barrier (cluster_before) before
-// any CTA exits.
-template <typename K, int THREADS>
-__device__ Cut<K> cluster_cut(const K* keys, int n, int target, K skip, uint32_t* top, CutShared<K, THREADS>& sh) {
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = cluster.num_blocks();
+// all others, and among themselves by row order; keys of 0 stand aside. The row
+// holds at least `target` keys that are not 0 (with fewer, all are taken).
+// Every thread of the row's CTAs calls it, after a __syncthreads behind the
+// writes of keys[0, n). It reads other CTAs' shared memory until it returns:
+// the caller passes a row barrier (row_before) before any CTA exits.
+template <typename K, int THREADS, bool LONE>
+__device__ Cut<K> row_cut(const K* keys, int n, int target, K skip, CutShared<K, THREADS, LONE>& sh) {
+    constexpr int kBits = CutShared<K, THREADS, LONE>::kBits, kBins = 1 << kBits, kWarps = THREADS / 32;
+    constexpr int kRanks = LONE ? 1 : kMaxCluster;
+    static_assert(kBins % THREADS == 0, "whole buckets per thread");
+    constexpr int kPer = kBins / THREADS;
+    const int ranks = LONE ? 1 : cooperative_groups::this_cluster().num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    static_assert(kCutBins % THREADS == 0, "whole buckets per thread");
-    constexpr int kPer = kCutBins / THREADS;
 
     K lo = ~(K)0, hi = 0;
     int firsts = 0, rest = 0;
@@ -70,48 +94,31 @@ __device__ Cut<K> cluster_cut(const K* keys, int n, int target, K skip, uint32_t
     }
     firsts = __reduce_add_sync(~0u, firsts);
     rest = __reduce_add_sync(~0u, rest);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        lo = min(lo, __shfl_xor_sync(~0u, lo, o));
-        hi = max(hi, __shfl_xor_sync(~0u, hi, o));
-    }
+    range_reduce(lo, hi);
     if (lane == 0) sh.warp_lo[warp] = lo, sh.warp_hi[warp] = hi, sh.warp_sum[warp] = firsts, sh.warp_rest[warp] = rest;
-    for (int i = tid; i < kCutBins; i += THREADS) sh.hist[0][i] = 0;
+    for (int i = tid; i < kBins; i += THREADS) sh.hist[0][i] = 0;
     __syncthreads();
-    if (warp == 0) {
-        lo = lane < THREADS / 32 ? sh.warp_lo[lane] : ~(K)0;
-        hi = lane < THREADS / 32 ? sh.warp_hi[lane] : 0;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            lo = min(lo, __shfl_xor_sync(~0u, lo, o));
-            hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+    lo = lane < kWarps ? sh.warp_lo[lane] : ~(K)0;
+    hi = lane < kWarps ? sh.warp_hi[lane] : 0;
+    firsts = __reduce_add_sync(~0u, lane < kWarps ? sh.warp_sum[lane] : 0);
+    rest = __reduce_add_sync(~0u, lane < kWarps ? sh.warp_rest[lane] : 0);
+    range_reduce(lo, hi);
+    if (!LONE) {
+        if (tid == 0) sh.range[0] = lo, sh.range[1] = hi, sh.counts = make_int2(firsts, rest);
+        row_sync<LONE>();
+        lo = ~(K)0, hi = 0, firsts = rest = 0;
+        if (lane < ranks) {
+            const K* remote = at_rank<LONE>(sh.range, lane);
+            lo = remote[0];
+            hi = remote[1];
+            const int2 c = *at_rank<LONE>(&sh.counts, lane);
+            firsts = c.x;
+            rest = c.y;
         }
-        firsts = __reduce_add_sync(~0u, lane < THREADS / 32 ? sh.warp_sum[lane] : 0);
-        rest = __reduce_add_sync(~0u, lane < THREADS / 32 ? sh.warp_rest[lane] : 0);
-        if (lane == 0) sh.range[0] = lo, sh.range[1] = hi, sh.counts = make_int2(firsts, rest), sh.top = *top;
+        firsts = __reduce_add_sync(~0u, firsts);
+        rest = __reduce_add_sync(~0u, rest);
+        range_reduce(lo, hi);
     }
-    cluster.sync();
-    lo = ~(K)0, hi = 0, firsts = rest = 0;
-    uint32_t most = 0;
-    if (lane < ranks) {
-        most = *cluster.map_shared_rank(&sh.top, lane);
-        const K* remote = cluster.map_shared_rank(sh.range, lane);
-        lo = remote[0];
-        hi = remote[1];
-        const int2 c = *cluster.map_shared_rank(&sh.counts, lane);
-        firsts = c.x;
-        rest = c.y;
-    }
-    firsts = __reduce_add_sync(~0u, firsts);
-    rest = __reduce_add_sync(~0u, rest);
-    *top = __reduce_max_sync(~0u, most);
-#pragma unroll
-    for (int o = kMaxCluster / 2; o; o >>= 1) {
-        lo = min(lo, __shfl_xor_sync(~0u, lo, o));
-        hi = max(hi, __shfl_xor_sync(~0u, hi, o));
-    }
-    lo = __shfl_sync(~0u, lo, 0);
-    hi = __shfl_sync(~0u, hi, 0);
 
     if (firsts > target) return {skip, ~(K)0, target, true};
     int want = min(target - firsts, rest);
@@ -119,31 +126,31 @@ __device__ Cut<K> cluster_cut(const K* keys, int n, int target, K skip, uint32_t
 
     for (int pass = 0;; ++pass) {
         int* hist = sh.hist[pass & 1];
+        int* found = sh.found[pass & 1];
         const int bits = bit_length((K)(hi - lo));
-        const int shift = bits > kCutBits ? bits - kCutBits : 0;
+        const int shift = bits > kBits ? bits - kBits : 0;
         for (int i = tid; i < n; i += THREADS) {
             const K k = keys[i];
             if (k >= lo && k <= hi) atomicAdd(&hist[(int)((k - lo) >> shift)], 1);
         }
-        cluster.sync();
+        row_sync<LONE>();
         // The other buffer is free again: all ranks have read it before this barrier.
-        for (int i = tid; i < kCutBins; i += THREADS) sh.hist[(pass + 1) & 1][i] = 0;
+        for (int i = tid; i < kBins; i += THREADS) sh.hist[(pass + 1) & 1][i] = 0;
         // Buckets from the top, kPer a thread.
-        int part[kMaxCluster][kPer], count[kPer], sum = 0;
+        int part[kRanks][kPer], count[kPer], sum = 0;
 #pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-            const int* remote = cluster.map_shared_rank(hist, r < ranks ? r : 0);
+        for (int r = 0; r < kRanks; ++r) {
+            const int* remote = at_rank<LONE>(hist, r < ranks ? r : 0);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) part[r][i] = r < ranks ? remote[kCutBins - 1 - (tid * kPer + i)] : 0;
+            for (int i = 0; i < kPer; ++i) part[r][i] = r < ranks ? remote[kBins - 1 - (tid * kPer + i)] : 0;
         }
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             count[i] = 0;
 #pragma unroll
-            for (int r = 0; r < kMaxCluster; ++r) count[i] += part[r][i];
+            for (int r = 0; r < kRanks; ++r) count[i] += part[r][i];
+            sum += count[i];
         }
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += count[i];
         int inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -152,24 +159,22 @@ __device__ Cut<K> cluster_cut(const K* keys, int n, int target, K skip, uint32_t
         }
         if (lane == 31) sh.warp_sum[warp] = inc;
         __syncthreads();
-        int above = inc - sum;
-        for (int w = 0; w < warp; ++w) above += sh.warp_sum[w];
+        int above = inc - sum + __reduce_add_sync(~0u, lane < warp ? sh.warp_sum[lane] : 0);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             if (above < want && want <= above + count[i]) {
-                sh.found[0] = kCutBins - 1 - (tid * kPer + i);
-                sh.found[1] = above;
-                sh.found[2] = count[i];
+                found[0] = kBins - 1 - (tid * kPer + i);
+                found[1] = above;
+                found[2] = count[i];
             }
             above += count[i];
         }
         __syncthreads();
-        const int bucket = sh.found[0], in_it = sh.found[2];
-        want -= sh.found[1];
-        lo = lo + ((K)bucket << shift);
+        const int in_it = found[2];
+        want -= found[1];
+        lo = lo + ((K)found[0] << shift);
         hi = lo + min((K)(hi - lo), (K)(((K)1 << shift) - 1));  // lo + 2^shift may not fit
         if (shift == 0 || in_it == want) return {lo, hi, want, in_it > want};
-        __syncthreads();  // found is read before the next pass writes it
     }
 }
 
@@ -186,10 +191,17 @@ __device__ __forceinline__ int warps_before(int mine, int* slots, int* all) {
     return __reduce_add_sync(~0u, lane < warp ? x : 0);
 }
 
-// What the cluster's ranks before this one hold of two values per CTA. Each
-// rank stores its own into the others' slots (kMaxCluster of them) ahead of
-// the barrier, so nothing reads another CTA's memory behind it.
-__device__ __forceinline__ int2 cluster_before(int2 mine, int2* slots) {
+// What the row's CTAs before this one hold of two values per CTA. Each rank
+// stores its own into the others' slots (kMaxCluster of them) ahead of the
+// barrier, so nothing reads another CTA's memory behind it.
+template <bool LONE>
+__device__ __forceinline__ int2 row_before(int2 mine, int2* slots) {
+    if (LONE) {
+        __syncthreads();
+        if (threadIdx.x == 0) slots[0] = mine;
+        __syncthreads();
+        return make_int2(0, 0);
+    }
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, ranks = cluster.num_blocks(), rank = cluster.block_rank();
