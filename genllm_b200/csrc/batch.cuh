@@ -94,6 +94,19 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Dynamic shared memory up to `bytes`; with `all` the SM's whole carveout, so
+// that a CTA of the kernel behind fits beside this one's. (Kernels that load
+// through L1 keep the driver's choice: page bounds took 17 us so, 22 with the
+// whole carveout.)
+template <typename Kernel>
+inline cudaError_t configure_kernel(Kernel kernel, size_t bytes, bool all = false) {
+    cudaError_t e = cudaSuccess;
+    if (bytes) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && all)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e;
+}
+
 // Launch as a programmatic dependent: the kernel waits (pdl_wait) before it
 // touches anything the kernels ahead of it on the stream write.
 template <typename... Args, typename... Given>

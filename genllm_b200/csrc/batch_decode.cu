@@ -507,154 +507,221 @@ __device__ __forceinline__ int units_of(const DecodeParams& p, int b) {
     return min(p.d.pages ? p.d.n_pages : 0x7FFFFFFF, pages_of(tokens));
 }
 
-// Joins the parts of each cut sequence, in order. An item is (segment, y): a
-// segment of at most 32 parts is joined by its first items, one row (query
-// head) a warp; a longer one by all, one row a CTA, its warps taking the parts
-// in turn. Bound: latency, two round trips to L2 behind the wait: nothing that
-// is loaded depends on the parts' maxima. (Folding with a running maximum, one
-// warp after the other, took 13 us on 147 parts.)
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
+__device__ __forceinline__ void store_lse(const DecodeParams& p, size_t q_row, float m, float l) {
+    const float e = m == -INFINITY ? -INFINITY : m + log2f(l);
+    p.lse2[q_row] = e;
+    if (p.d.lse) p.d.lse[q_row] = e * kLn2;
+}
+
+// Joins the parts of each cut sequence, in order. A segment of at most 32
+// parts is joined one row (query head) a warp, a longer one one row a CTA; when
+// these are few (one long sequence), a quarter of a row's dims a CTA, so that
+// its parts (2.4 MB at 32 heads and 147 parts) are fetched by many SMs. Bound:
+// latency. Everything but the loads comes before the wait for the decode
+// kernel, no load depends on another, and each maximum and sum is loaded once a
+// CTA: once a warp took 4000 cycles, all of them asking the same few lines of
+// L2. 72 registers, so that a CTA fits beside one of the decode kernel.
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kJoinCuts = 4, kFewParts = 32;
+constexpr int kMaxParts = kMaxGrid * 8;
+
+struct JoinShared {
+    int warp_sums[32];
+    int slots[kJoinWarps];
+    int cut_segs[kMaxParts];  // segments: those of few parts from the front, the others from the back
+    float2 ml[kMaxParts];     // of one row's parts
+    float4 acc[kJoinWarps][64];
+};
+
+// One row's dims [cut * D / CUTS, + D / CUTS) from its `parts` parts, by the CTA.
+template <int D, int CUTS, typename Slot>
+__device__ __forceinline__ void join_many(const DecodeParams& p, JoinShared& sh, int parts, Slot slot, size_t q_row, int cut) {
+    constexpr int kSpan = D / CUTS, kLanes = kSpan / 4 < 32 ? kSpan / 4 : 32;  // lanes of a part's span
+    constexpr int kVecs = kSpan / 4 / kLanes;          // 16-byte loads of a lane and part
+    constexpr int kStep = kJoinWarps * (32 / kLanes);  // parts of the CTA's one load
+    constexpr int kBatch = 5;                          // parts of a lane in flight
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part0 = warp * (32 / kLanes) + lane / kLanes;
+    const size_t dims = cut * kSpan + (lane % kLanes) * 4;
+    float4 x[kBatch][kVecs], acc[kVecs];
+    auto load = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j) {
+                const int i = from + k * kStep;
+                x[k][j] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * D + dims + j * kLanes * 4)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    };
+    load(part0);
+    for (int i = threadIdx.x; i < parts; i += kJoinThreads) sh.ml[i] = p.part_ml[slot(i)];
+    __syncthreads();
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, sh.ml[i].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    auto factor_of = [&](float part_m) { return part_m == m ? 1.f : exp2_of(part_m - m); };
+    float l = 0.f;
+    for (int i = lane; i < parts; i += 32) l += sh.ml[i].y * factor_of(sh.ml[i].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = part0;;) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float f = i + k * kStep < parts ? factor_of(sh.ml[i + k * kStep].x) : 0.f;
+#pragma unroll
+            for (int j = 0; j < kVecs; ++j) {
+                acc[j].x += x[k][j].x * f;
+                acc[j].y += x[k][j].y * f;
+                acc[j].z += x[k][j].z * f;
+                acc[j].w += x[k][j].w * f;
+            }
+        }
+        i += kBatch * kStep;
+        if (i - part0 >= parts) break;
+        load(i);
+    }
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+#pragma unroll
+        for (int o = kLanes; o < 32; o <<= 1) {
+            acc[j].x += __shfl_xor_sync(~0u, acc[j].x, o);
+            acc[j].y += __shfl_xor_sync(~0u, acc[j].y, o);
+            acc[j].z += __shfl_xor_sync(~0u, acc[j].z, o);
+            acc[j].w += __shfl_xor_sync(~0u, acc[j].w, o);
+        }
+        if (lane < kLanes) sh.acc[warp][j * kLanes + lane] = acc[j];
+    }
+    __syncthreads();
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key at all: zeros
+    if (threadIdx.x < kSpan) {
+        float o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) o += reinterpret_cast<const float*>(sh.acc[w])[threadIdx.x];
+        store_out(p.d.out, q_row * D + cut * kSpan + threadIdx.x, o * inv, p.d.out_dtype);
+    }
+    if (cut == 0 && threadIdx.x == 0) store_lse(p, q_row, m, l);
+    __syncthreads();
+}
+
+// One row by a warp: lane i holds part i's factor.
+template <int D, typename Slot>
+__device__ __forceinline__ void join_few(const DecodeParams& p, int parts, Slot slot, size_t q_row) {
+    constexpr int kPer = D / 32, kBatch = D == 256 ? 4 : 8;
+    const int lane = threadIdx.x & 31;
+    const float2 ml = lane < parts ? p.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+    float2 x[kBatch][kPer / 2], acc[kPer / 2];
+    auto load = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int j = 0; j < kPer / 2; ++j)
+                x[k][j] = from + k < parts
+                              ? reinterpret_cast<const float2*>(p.part_acc + slot(from + k) * D + lane * kPer)[j]
+                              : make_float2(0.f, 0.f);
+    };
+    load(0);
+    float m = ml.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const float c = ml.x == m ? 1.f : exp2_of(ml.x - m);
+    float l = lane < parts ? ml.y * c : 0.f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+    for (int i = 0;;) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const float f = __shfl_sync(~0u, c, i + k);
+#pragma unroll
+            for (int j = 0; j < kPer / 2; ++j) {
+                acc[j].x += i + k < parts ? x[k][j].x * f : 0.f;
+                acc[j].y += i + k < parts ? x[k][j].y * f : 0.f;
+            }
+        }
+        i += kBatch;
+        if (i >= parts) break;
+        load(i);
+    }
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) {
+        store_out(p.d.out, q_row * D + lane * kPer + 2 * j, acc[j].x * inv, p.d.out_dtype);
+        store_out(p.d.out, q_row * D + lane * kPer + 2 * j + 1, acc[j].y * inv, p.d.out_dtype);
+    }
+    if (lane == 0) store_lse(p, q_row, m, l);
+}
+
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads, 2) batch_join_kernel(const DecodeParams p) {
-    constexpr int kPer = D / 32;                  // dims of a lane, neighbours
-    constexpr int kBatch = D == 256 ? 10 : 20;    // parts of a warp in flight
-    constexpr int kFactors = kMaxGrid * 8;
-    constexpr int kRounds = (kFactors + kJoinThreads - 1) / kJoinThreads;
+__global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
     extern __shared__ int base[];
-    __shared__ int warp_sums[32];
-    __shared__ float factor[kFactors];  // of all parts
-    __shared__ float sh_acc[kJoinWarps][D];
-    __shared__ float2 sh_ml[kJoinWarps];
-    scan_counts(p.v.batch, base, warp_sums, [&](int b) { return units_of(p, b); });
+    __shared__ JoinShared sh;
+    scan_counts(p.v.batch, base, sh.warp_sums, [&](int b) { return units_of(p, b); });
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rows = p.s.heads * p.group;
-    const int segments = p.v.batch * p.s.groups;
     const int total = base[p.v.batch] * p.s.groups;
     const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
-    pdl_wait();
-    pdl_trigger();
-    for (int64_t item = blockIdx.x; item < (int64_t)segments * rows; item += gridDim.x) {
-        const int y = (int)(item / segments), seg = (int)(item - (int64_t)y * segments);
+    // A cut segment belongs to the first boundary between workers inside it.
+    int n_few = 0, n_many = 0;
+    for (int w = 0; (int64_t)(w + 1) * per < total; w += kJoinThreads) {
+        const int64_t u = (int64_t)(w + (int)threadIdx.x + 1) * per;  // the boundary's unit
+        int seg = 0, parts = 0;
+        if (u < total) {
+            const int b = owner(base, p.v.batch, p.s.groups, (int)u);
+            const int count = base[b + 1] - base[b], grp = ((int)u - base[b] * p.s.groups) / count;
+            const int s0 = base[b] * p.s.groups + grp * count;
+            seg = b * p.s.groups + grp;
+            if (s0 < u && s0 >= u - per) parts = (s0 + count - 1) / per - (w + (int)threadIdx.x) + 1;
+        }
+        const bool few = parts && parts <= kFewParts, many = parts > kFewParts;
+        const uint32_t few_mask = __ballot_sync(~0u, few), many_mask = __ballot_sync(~0u, many);
+        __syncthreads();
+        if (lane == 0) sh.slots[warp] = __popc(few_mask) | __popc(many_mask) << 16;
+        __syncthreads();
+        const int x = lane < kJoinWarps ? sh.slots[lane] : 0;
+        const int before = __reduce_add_sync(~0u, lane < warp ? x : 0), all = __reduce_add_sync(~0u, x);
+        const uint32_t below = (1u << lane) - 1;
+        if (few) sh.cut_segs[n_few + (before & 0xFFFF) + __popc(few_mask & below)] = seg;
+        if (many) sh.cut_segs[kMaxParts - 1 - (n_many + (before >> 16) + __popc(many_mask & below))] = seg;
+        n_few += all & 0xFFFF;
+        n_many += all >> 16;
+    }
+    __syncthreads();
+    const int few_blocks = (rows + kJoinWarps - 1) / kJoinWarps;
+    const int cuts = n_many * rows * kJoinCuts <= (int)gridDim.x ? kJoinCuts : 1;
+    const int few_items = n_few * few_blocks, items = few_items + n_many * rows * cuts;
+    bool waited = false;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const bool few = item < few_items;
+        const int at = few ? item / few_blocks : (item - few_items) / (rows * cuts);
+        const int y = few ? item - at * few_blocks : item - few_items - at * rows * cuts;
+        const int seg = sh.cut_segs[few ? at : kMaxParts - 1 - at];
         const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
         const int count = base[b + 1] - base[b];
-        if (count == 0) continue;
-        const int s0 = base[b] * p.s.groups + grp * count, s1 = s0 + count;
-        const int w0 = s0 / per, w1 = (s1 - 1) / per, parts = w1 - w0 + 1;
-        if (parts == 1) continue;
-        const bool one_warp = parts <= 32;
-        const int row = one_warp ? y * kJoinWarps + warp : y;
-        const bool there = row < rows && grp * p.s.heads + row / p.group < p.v.hkv;
-        if (!there) continue;
+        const int s0 = base[b] * p.s.groups + grp * count, w0 = s0 / per, parts = (s0 + count - 1) / per - w0 + 1;
+        const int row = few ? y * kJoinWarps + warp : y / cuts;
+        if (row >= rows || grp * p.s.heads + row / p.group >= p.v.hkv) continue;
         // Part i lies in its worker's first slot, the segment's first part in the second unless it starts the worker's.
-        auto slot = [&](int i) {
-            return (size_t)(2 * (w0 + i) + (i == 0 && s0 != w0 * per ? 1 : 0)) * rows + row;
-        };
-        const int first = one_warp ? 0 : warp, step = one_warp ? 1 : kJoinWarps;
-        float x[kBatch][kPer], acc[kPer];
-        auto load = [&](int from) {
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const int i = from + k * step;
-                const float* at = p.part_acc + slot(min(i, parts - 1)) * D + lane * kPer;
-#pragma unroll
-                for (int j = 0; j < kPer; j += 2) {
-                    const float2 v2 = i < parts ? *reinterpret_cast<const float2*>(at + j) : make_float2(0.f, 0.f);
-                    x[k][j] = v2.x, x[k][j + 1] = v2.y;
-                }
-            }
-        };
-        auto add = [&](int from, auto factor_of) {
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const float c = factor_of(min(from + k * step, parts - 1));
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) acc[j] += x[k][j] * c;
-            }
-        };
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
-        load(first);
+        const size_t slot0 = (size_t)2 * w0 * rows + row;
+        const int shift0 = s0 != w0 * per ? rows : 0;
+        auto slot = [&](int i) { return slot0 + (size_t)(2 * i) * rows + (i == 0 ? shift0 : 0); };
         const size_t q_row = (size_t)b * p.d.n_q_heads + grp * rows + row;
-        if (one_warp) {
-            const float2 ml = lane < parts ? p.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
-            float m = ml.x;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-            const float c = ml.x == m ? 1.f : exp2_of(ml.x - m);
-            float l = ml.y * c;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-            auto factor_of = [&](int i) { return __shfl_sync(~0u, c, i); };
-            add(0, factor_of);
-            for (int i = kBatch; i < parts; i += kBatch) {
-                load(i);
-                add(i, factor_of);
-            }
-            const bool none = m == -INFINITY;  // no key at all
-            const float inv = none ? 0.f : 1.f / l;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) store_out(p.d.out, q_row * D + lane * kPer + j, acc[j] * inv, p.d.out_dtype);
-            if (lane == 0) {
-                const float e = none ? -INFINITY : m + log2f(l);
-                p.lse2[q_row] = e;
-                if (p.d.lse) p.d.lse[q_row] = e * kLn2;
-            }
-            continue;
+        if (!waited) {
+            pdl_wait();
+            pdl_trigger();
+            waited = true;
         }
-        float m = -INFINITY;
-        float2 ml[kRounds];
-#pragma unroll
-        for (int k = 0; k < kRounds; ++k) {
-            const int i = k * kJoinThreads + threadIdx.x;
-            ml[k] = i < parts ? p.part_ml[slot(i)] : make_float2(-INFINITY, 0.f);
-            m = fmaxf(m, ml[k].x);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        if (lane == 0) sh_ml[warp].x = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sh_ml[w].x);
-        float l = 0.f;
-#pragma unroll
-        for (int k = 0; k < kRounds; ++k) {
-            const int i = k * kJoinThreads + threadIdx.x;
-            if (i < parts) {
-                const float c = ml[k].x == m ? 1.f : exp2_of(ml[k].x - m);
-                factor[i] = c;
-                l += ml[k].y * c;
-            }
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-        if (lane == 0) sh_ml[warp].y = l;
-        __syncthreads();
-        auto factor_of = [&](int i) { return factor[i]; };
-        add(first, factor_of);
-        for (int i = first + step * kBatch; i < parts; i += step * kBatch) {
-            load(i);
-            add(i, factor_of);
-        }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) sh_acc[warp][lane * kPer + j] = acc[j];
-        __syncthreads();
-        l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) l += sh_ml[w].y;
-        const bool none = m == -INFINITY;
-        const float inv = none ? 0.f : 1.f / l;
-        for (int d = threadIdx.x; d < D; d += kJoinThreads) {
-            float o = 0.f;
-#pragma unroll
-            for (int w = 0; w < kJoinWarps; ++w) o += sh_acc[w][d];
-            store_out(p.d.out, q_row * D + d, o * inv, p.d.out_dtype);
-        }
-        if (threadIdx.x == 0) {
-            const float e = none ? -INFINITY : m + log2f(l);
-            p.lse2[q_row] = e;
-            if (p.d.lse) p.d.lse[q_row] = e * kLn2;
-        }
-        __syncthreads();
+        if (few) join_few<D>(p, parts, slot, q_row);
+        else if (cuts == 1) join_many<D, 1>(p, sh, parts, slot, q_row, 0);
+        else join_many<D, kJoinCuts>(p, sh, parts, slot, q_row, y % cuts);
+    }
+    // Every CTA waits, so that this kernel ends behind the decode kernel.
+    if (!waited) {
+        pdl_wait();
+        pdl_trigger();
     }
 }
 
@@ -753,13 +820,14 @@ cudaError_t configure_batch_decode() {
     for (int f16 = 0; f16 < 2; ++f16)
         for (int dim = 64; dim <= 256; dim *= 2)
             for (int two = 0; two < 2; ++two) {
-                cudaError_t e = for_kernel(f16, dim, two, [](auto* k) {
-                    return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                (int)smem_bytes(kMaxBatch));
-                });
+                const cudaError_t e =
+                    for_kernel(f16, dim, two, [](auto* k) { return configure_kernel(k, smem_bytes(kMaxBatch), true); });
                 if (e != cudaSuccess) return e;
             }
-    return cudaSuccess;
+    cudaError_t e = configure_kernel(batch_join_kernel<64>, 0, true);
+    if (e == cudaSuccess) e = configure_kernel(batch_join_kernel<128>, 0, true);
+    if (e == cudaSuccess) e = configure_kernel(batch_join_kernel<256>, 0, true);
+    return e;
 }
 
 cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, cudaStream_t stream) {
@@ -781,8 +849,9 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
     if (e != cudaSuccess) return e;
     // The join is always launched: it also keeps the launches behind it from
     // starting before the appended rows are in their pages.
-    const int64_t items = (int64_t)v.batch * p.s.groups * p.s.heads * p.group;
-    const dim3 grid((unsigned)std::min<int64_t>(items, (int64_t)v.sms * 8));
+    // At most what runs at once: a second wave would start behind the first.
+    const int items = v.batch * p.s.groups * p.s.heads * p.group * kJoinCuts;
+    const dim3 grid((unsigned)std::min(items, v.sms));
     const size_t base_bytes = sizeof(int) * (size_t)(v.batch + 1);
     e = v.dim == 64    ? launch_dependent(batch_join_kernel<64>, grid, dim3(kJoinThreads), base_bytes, stream, p)
         : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinThreads), base_bytes, stream, p)

@@ -262,11 +262,8 @@ EvictSpace evict_space(const BatchView& v) {
 size_t evict_bytes(const BatchView& v) { return evict_space(v).all; }
 
 cudaError_t configure_evict() {
-    const int most = kMaxSlice * (int)sizeof(uint32_t);
-    const cudaError_t e = cudaFuncSetAttribute(evict_plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    return e != cudaSuccess
-               ? e
-               : cudaFuncSetAttribute(evict_plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    const cudaError_t e = configure_kernel(evict_plan_kernel<true>, kMaxSlice * sizeof(uint32_t));
+    return e != cudaSuccess ? e : configure_kernel(evict_plan_kernel<false>, kMaxSlice * sizeof(uint32_t));
 }
 
 cudaError_t launch_evict(const BatchView& v, const EvictLaunch& e, cudaStream_t stream) {

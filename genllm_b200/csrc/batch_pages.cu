@@ -583,11 +583,9 @@ struct LaunchSelect {
 struct ConfigureSelect {
     template <bool F16, int D>
     cudaError_t operator()() const {
-        const int most = kMaxSlice * (int)sizeof(uint32_t);
-        const cudaError_t e = cudaFuncSetAttribute(page_pick_kernel<F16, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        return e != cudaSuccess ? e
-                                : cudaFuncSetAttribute(page_pick_kernel<F16, D, false>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        constexpr size_t kMost = kMaxSlice * sizeof(uint32_t);
+        const cudaError_t e = configure_kernel(page_pick_kernel<F16, D, true>, kMost);
+        return e != cudaSuccess ? e : configure_kernel(page_pick_kernel<F16, D, false>, kMost);
     }
 };
 
