@@ -726,35 +726,56 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
 }
 
 // weights_out[t] = decay * weights_in[t] + sum over the head's queries of
-// exp2(s_t - lse): a thread per token, over a line of 256-token chunks of all
-// (sequence, head) rows. Bound: HBM and L2, 4 G + 8 bytes a token and head.
-constexpr int kTotalsThreads = 256;
+// exp2(s_t - lse): a CTA per chunk of 1024 tokens of one (sequence, head), four
+// tokens a thread in flight. Bound: HBM and L2, 4 G + 8 bytes a token and head.
+constexpr int kTotalsThreads = 256, kTotalsTokens = 4, kTotalsChunk = kTotalsThreads * kTotalsTokens;
+template <int V>  // scores of one load: the group is a multiple of it
 __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const DecodeParams p) {
+    struct __align__(V * 4) Vec {
+        float x[V];
+    };
     extern __shared__ int chunks[];
     __shared__ int warp_sums[32];
     const int G = p.group, hkv = p.v.hkv;
-    constexpr int kPages = kTotalsThreads / kPageSlots;
+    constexpr int kPages = kTotalsChunk / kPageSlots;
     // Chunks before each sequence, and units.
     int* base = chunks + p.v.batch + 1;
-    scan_counts(p.v.batch, chunks, warp_sums, [&](int b) { return (units_of(p, b) + kPages - 1) / kPages; });
-    __syncthreads();
     scan_counts(p.v.batch, base, warp_sums, [&](int b) { return units_of(p, b); });
+    __syncthreads();
+    scan_counts(p.v.batch, chunks, warp_sums, [&](int b) { return (base[b + 1] - base[b] + kPages - 1) / kPages; });
     pdl_wait();
     pdl_trigger();
     const int64_t all = (int64_t)chunks[p.v.batch] * hkv;
     for (int64_t c = blockIdx.x; c < all; c += gridDim.x) {
         const int at = (int)(c / hkv), h = (int)(c - (int64_t)at * hkv);
         const int b = owner(chunks, p.v.batch, 1, at);
-        const int t = (at - chunks[b]) * kTotalsThreads + threadIdx.x;
-        const int n = attended(p.v, p.d, b, false);
-        if (t >= n) continue;
-        const size_t place = ((size_t)b * hkv + h) * p.d.weights_stride + t;
-        const float old = p.d.weights_in && t < p.v.lens[b] ? p.d.decay * p.d.weights_in[place] : 0.f;
-        const float* s = p.scores + (((size_t)base[b] * hkv + (size_t)h * (base[b + 1] - base[b])) * kPageSlots + t) * G;
+        const int t0 = (at - chunks[b]) * kTotalsChunk + threadIdx.x;
+        const int units = base[b + 1] - base[b];
+        const int len = p.v.lens[b], n = attended(p.v, p.d, b, false);
+        const size_t row = ((size_t)b * hkv + h) * p.d.weights_stride;
+        const float* s = p.scores + ((size_t)base[b] * hkv + (size_t)h * units) * kPageSlots * G;
         const float* e = p.lse2 + (size_t)b * p.d.n_q_heads + h * G;
-        float sum = 0.f;
-        for (int g = 0; g < G; ++g) sum += exp2_of(s[g] - e[g]);
-        p.d.weights_out[place] = old + sum;
+        float sum[kTotalsTokens];
+#pragma unroll
+        for (int i = 0; i < kTotalsTokens; ++i) {
+            const int t = t0 + i * kTotalsThreads;
+            sum[i] = p.d.weights_in && t < min(n, len) ? p.d.decay * p.d.weights_in[row + t] : 0.f;
+        }
+        for (int g = 0; g < G; g += V) {
+            Vec x[kTotalsTokens];
+#pragma unroll
+            for (int i = 0; i < kTotalsTokens; ++i)
+                x[i] = *reinterpret_cast<const Vec*>(s + (size_t)min(t0 + i * kTotalsThreads, units * kPageSlots - 1) * G + g);
+#pragma unroll
+            for (int i = 0; i < kTotalsTokens; ++i)
+#pragma unroll
+                for (int k = 0; k < V; ++k) sum[i] += exp2_of(x[i].x[k] - e[g + k]);
+        }
+#pragma unroll
+        for (int i = 0; i < kTotalsTokens; ++i) {
+            const int t = t0 + i * kTotalsThreads;
+            if (t < n) p.d.weights_out[row + t] = sum[i];
+        }
     }
 }
 
@@ -857,8 +878,10 @@ cudaError_t launch_batch_decode(const BatchView& v, const BatchDecodeLaunch& d, 
         : v.dim == 128 ? launch_dependent(batch_join_kernel<128>, grid, dim3(kJoinThreads), base_bytes, stream, p)
                        : launch_dependent(batch_join_kernel<256>, grid, dim3(kJoinThreads), base_bytes, stream, p);
     if (e != cudaSuccess || !d.weights_out) return e;
-    return launch_dependent(batch_totals_kernel, dim3(v.sms * 8), dim3(kTotalsThreads),
-                            sizeof(int) * (size_t)(2 * v.batch + 2), stream, p);
+    auto* totals = p.group % 4 == 0   ? batch_totals_kernel<4>
+                   : p.group % 2 == 0 ? batch_totals_kernel<2>
+                                      : batch_totals_kernel<1>;
+    return launch_dependent(totals, dim3(v.sms * 4), dim3(kTotalsThreads), sizeof(int) * (size_t)(2 * v.batch + 2), stream, p);
 }
 
 }  // namespace gkv

@@ -159,9 +159,9 @@ constexpr float kScoreError = 2 * (D / 8) * 18 * 0x1p-23f;
 constexpr float kTiny = 0x1p-117f;
 constexpr uint32_t kKeyInf = 0xFF800000u, kKeyMinusInf = 0x007FFFFFu;  // key32_of the infinities
 
-// The score of one page in fp64, by a whole warp.
+// The score of one page in fp64, by a whole warp; queries: [group][D] in shared memory.
 template <bool F16, int D>
-__device__ uint64_t exact_key(const SelectParams& p, int b, int h, int page) {
+__device__ uint64_t exact_key(const SelectParams& p, int h, int page, const float* queries) {
     constexpr int kPer = D / 32;
     const int lane = threadIdx.x & 31;
     const uint16_t* lo = p.s.bounds + ((size_t)page * p.v.hkv + h) * 2 * D + lane * kPer;
@@ -174,15 +174,12 @@ __device__ uint64_t exact_key(const SelectParams& p, int b, int h, int page) {
     }
     double best = -INFINITY;
     bool nan = false;
+#pragma unroll 4
     for (int g = 0; g < p.group; ++g) {
-        const uint16_t* q = p.s.q + b * p.s.q_stride_batch + (int64_t)(h * p.group + g) * p.s.q_stride_head + lane * kPer;
+        const float* q = queries + g * D + lane * kPer;
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-            const float2 a = floats_of<F16>(*reinterpret_cast<const uint32_t*>(q + i));
-            sum += (double)a.x * (double)(a.x >= 0.f ? x[i] : l[i]);
-            sum += (double)a.y * (double)(a.y >= 0.f ? x[i + 1] : l[i + 1]);
-        }
+        for (int i = 0; i < kPer; ++i) sum += (double)q[i] * (double)(q[i] >= 0.f ? x[i] : l[i]);
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
         nan |= sum != sum;
@@ -330,7 +327,8 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         uint64_t key;
         int page;
     };
-    extern __shared__ uint32_t slice_keys[];
+    extern __shared__ __align__(16) float queries[];  // [group][D], and behind them the slice's keys
+    uint32_t* slice_keys = reinterpret_cast<uint32_t*>(queries + p.group * D);
     __shared__ union {
         CutShared<uint32_t, kPickThreads, LONE> approx;
         CutShared<uint64_t, kPickThreads, LONE> exact;
@@ -356,6 +354,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
                                                                 (int64_t)(h * p.group + g) * p.s.q_stride_head);
         for (int d = lane; d < D / 2; d += 32) {
             const float2 x = floats_of<F16>(__ldcg(row + d));
+            *reinterpret_cast<float2*>(queries + g * D + 2 * d) = x;
             sum += fabsf(x.x) + fabsf(x.y);
         }
 #pragma unroll
@@ -376,6 +375,9 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     const int p0 = min(pages, rank * slice), m = min(pages - p0, slice);
     const int2* table = v.table + b * v.table_stride;
     uint32_t* keys = p.approx + (size_t)bh * v.table_pages + p0;
+    // Every CTA looks at all tiles' largest bounds.
+    const int max_tiles = (v.table_pages + 15) / 16;
+    uint32_t top = tid < (pages + 15) / 16 ? p.tops[(size_t)bh * max_tiles + tid] : 0;
     if (!p.spill) {
         for (int i = tid; i < m; i += 8 * kPickThreads) {
             uint32_t x[8];
@@ -387,10 +389,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         }
         keys = slice_keys;
     }
-    // Every CTA looks at all tiles' largest bounds.
-    const int max_tiles = (v.table_pages + 15) / 16;
-    uint32_t top = 0;
-    for (int i = tid; i < (pages + 15) / 16; i += kPickThreads) top = max(top, p.tops[(size_t)bh * max_tiles + i]);
+    for (int i = tid + kPickThreads; i < (pages + 15) / 16; i += kPickThreads) top = max(top, p.tops[(size_t)bh * max_tiles + i]);
     top = __reduce_max_sync(~0u, top);
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
@@ -456,7 +455,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         __syncthreads();
         for (int i = before.y + warp; i < before.y + cut_all; i += kPickWarps) {
             const int lp = close_page[i], page = table[lp].x;
-            const uint64_t key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, b, h, page);
+            const uint64_t key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, h, page, queries);
             if (lane < ranks) {
                 Close* remote = at_rank<LONE>(close, lane);
                 remote[i].key = key;
@@ -490,7 +489,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         uint64_t key = k > in ? kTaken : 0;
         if (k >= out && k <= in) {
             const int page = table[p0 + i].x;
-            key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, b, h, page);
+            key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, h, page, queries);
         }
         if (lane == 0) exact[i] = key;
     }
@@ -578,13 +577,13 @@ struct LaunchSelect {
         if (e != cudaSuccess) return e;
         return launch_cluster(s.cluster == 1 ? page_pick_kernel<F16, D, true> : page_pick_kernel<F16, D, false>,
                               (unsigned)(p.v.batch * p.v.hkv), s.cluster, kPickThreads,
-                              s.spill ? 0 : s.slice * sizeof(uint32_t), stream, q);
+                              sizeof(float) * p.group * D + (s.spill ? 0 : s.slice * sizeof(uint32_t)), stream, q);
     }
 };
 struct ConfigureSelect {
     template <bool F16, int D>
     cudaError_t operator()() const {
-        constexpr size_t kMost = kMaxSlice * sizeof(uint32_t);
+        constexpr size_t kMost = kMaxSlice * sizeof(uint32_t) + sizeof(float) * kMaxBatchGroup * D;
         const cudaError_t e = configure_kernel(page_pick_kernel<F16, D, true>, kMost);
         return e != cudaSuccess ? e : configure_kernel(page_pick_kernel<F16, D, false>, kMost);
     }
