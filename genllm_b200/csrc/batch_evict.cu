@@ -29,13 +29,13 @@ struct EvictParams {
     EvictLaunch e;
     int32_t* counts;   // [batch * hkv] moves of each head
     int32_t* left;     // [batch] new length, -1: skipped
-    Move* moves;       // [batch * hkv][16 * table_pages]
+    Move* moves;       // [batch * hkv][8 * table_pages]: a head moves at most half its slots
     uint32_t* keys;    // [batch * hkv][16 * table_pages] where a slice does not fit in shared memory; else null
 };
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kBatch = 8;          // loads of a thread in flight
+constexpr int kBatch = 12;         // slots of a thread loaded at once
 constexpr int kMaxSlice = 40960;  // keys of a CTA in shared memory: 160 KB
 constexpr uint32_t kRecent = ~0u, kNaN32 = ~0u - 1;
 
@@ -90,29 +90,32 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     const int slice = ((n + ranks - 1) / ranks + 31) / 32 * 32;
     const int s0 = min(n, rank * slice), m = min(n - s0, slice);
     uint32_t* keys = p.keys ? p.keys + (size_t)bh * cap + s0 : slice_keys;
-    for (int i = tid; i < m; i += kBatch * kPlanThreads) {
-        // All loads of a batch first: the row comes from HBM.
-        float w[kBatch];
-        int at[kBatch];
+    // A warp's run of the slice; its lanes' weights and positions, all loads of a
+    // batch first. A run of one batch keeps them until the end.
+    const int run = ((m + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+    const int i0 = min(m, warp * run), i1 = min(m, i0 + run);
+    const bool one_batch = run <= 32 * kBatch;
+    float w[kBatch];
+    int pos[kBatch];
+    auto load = [&](int ib) {
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int t = s0 + min(i + j * kPlanThreads, m - 1);
-            w[j] = weights[t];
-            at[j] = position(t);
+            const int i = ib + j * 32 + lane;
+            w[j] = i < i1 ? weights[s0 + i] : 0.f;
+            pos[j] = i < i1 ? position(s0 + i) : 0;
         }
+    };
+    for (int ib = i0; ib < i1; ib += 32 * kBatch) {
+        load(ib);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            if (i + j * kPlanThreads >= m) break;
-            const bool is_recent = at[j] >= seen - p.e.n_recent;
-            keys[i + j * kPlanThreads] = is_recent ? kRecent : key_of(w[j]);
+            const int i = ib + j * 32 + lane;
+            if (i < i1) keys[i] = pos[j] >= seen - p.e.n_recent ? kRecent : key_of(w[j]);
         }
     }
     __syncthreads();
     const Cut<uint32_t> cut = row_cut<uint32_t, kPlanThreads, LONE>(keys, m, left, kRecent, cut_shared);
 
-    // A warp's run of the slice.
-    const int run = ((m + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
-    const int i0 = min(m, warp * run), i1 = min(m, i0 + run);
     const uint32_t below = (1u << lane) - 1;
     int equal = 0;  // keys of the cut's range before this run, in slot order
     if (cut.partial) {
@@ -151,17 +154,10 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
         // The last run's end: the count of the whole row.
         p.counts[bh] = hole_at + holes;
     }
-    Move* moves = p.moves + (size_t)bh * cap;
+    Move* moves = p.moves + (size_t)bh * (cap / 2);
     at = equal;
     for (int ib = i0; ib < i1; ib += 32 * kBatch) {
-        float w[kBatch];
-        int pos[kBatch];
-#pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int t = s0 + min(ib + j * 32 + lane, m - 1);
-            w[j] = weights[t];
-            pos[j] = position(t);
-        }
+        if (!one_batch) load(ib);
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
             const int i = ib + j * 32;
@@ -199,7 +195,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
     const int left = p.left[b], count = p.counts[bh];
     if (left < 0) return;
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) p.e.lens_out[b] = left;
-    const Move* moves = p.moves + (size_t)bh * v.table_pages * kPageSlots;
+    const Move* moves = p.moves + (size_t)bh * v.table_pages * (kPageSlots / 2);
     const int2* table = v.table + b * v.table_stride;
     const int step = gridDim.x * (kMoveThreads / 32) * kGroup;
     for (int i0 = (blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5)) * kGroup; i0 < count; i0 += step) {
@@ -252,7 +248,7 @@ EvictSpace evict_space(const BatchView& v) {
     s.spill = (cap + s.cluster - 1) / s.cluster > kMaxSlice;
     s.left = round16(heads * sizeof(int32_t));
     s.moves = s.left + round16((size_t)v.batch * sizeof(int32_t));
-    s.keys = s.moves + heads * cap * sizeof(Move);
+    s.keys = s.moves + heads * (cap / 2) * sizeof(Move);
     s.all = s.keys + (s.spill ? heads * cap * sizeof(uint32_t) : 0);
     return s;
 }

@@ -145,8 +145,6 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 constexpr int kScoreWarps = 8;
-constexpr int kPickThreads = 512;
-constexpr int kPickWarps = kPickThreads / 32;
 constexpr int kMaxSlice = 16384;  // keys of a CTA in shared memory: 64 KB
 constexpr int kMaxClose = 64;     // pages at the cut that are ranked in shared memory
 
@@ -321,8 +319,9 @@ __global__ void __launch_bounds__(kScoreWarps * 32, NT == 1 && D <= 128 ? 2 : 1)
 
 // The taken pages of each (sequence, head) in rising order, one CTA or cluster
 // a row. Bound: latency (a chain of barriers over a few kilobytes).
-template <bool F16, int D, bool LONE>
-__global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectParams p) {
+template <bool F16, int D, bool LONE, int THREADS>
+__global__ void __launch_bounds__(THREADS) page_pick_kernel(const SelectParams p) {
+    constexpr int kWarps = THREADS / 32;
     struct Close {
         uint64_t key;
         int page;
@@ -330,14 +329,14 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     extern __shared__ __align__(16) float queries[];  // [group][D], and behind them the slice's keys
     uint32_t* slice_keys = reinterpret_cast<uint32_t*>(queries + p.group * D);
     __shared__ union {
-        CutShared<uint32_t, kPickThreads, LONE> approx;
-        CutShared<uint64_t, kPickThreads, LONE> exact;
+        CutShared<uint32_t, THREADS, LONE> approx;
+        CutShared<uint64_t, THREADS, LONE> exact;
     } cut_shared;
     __shared__ Close close[kMaxClose];
     __shared__ int close_page[kMaxClose];
-    __shared__ int slots[kPickWarps];
+    __shared__ int slots[kWarps];
     __shared__ int2 rank_slots[3][kMaxCluster];
-    __shared__ uint32_t warp_top[kPickWarps];
+    __shared__ uint32_t warp_top[kWarps];
     __shared__ float head_sum[kMaxBatchGroup];
     const BatchView& v = p.v;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -348,7 +347,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     // this one start once they are done), past L1.
     const int len = __ldcg(v.lens + b), cap = v.table_pages * kPageSlots;
     const int pages = len < 0 ? 0 : pages_of(min(len, cap - p.s.extra) + p.s.extra);
-    for (int g = warp; g < p.group; g += kPickWarps) {
+    for (int g = warp; g < p.group; g += kWarps) {
         float sum = 0.f;
         const uint32_t* row = reinterpret_cast<const uint32_t*>(p.s.q + b * p.s.q_stride_batch +
                                                                 (int64_t)(h * p.group + g) * p.s.q_stride_head);
@@ -366,9 +365,9 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     if (len < 0) return;  // the whole row
     int32_t* to = p.s.pages + (size_t)bh * p.s.n_pages;
     const int take = min(p.s.n_pages, pages);
-    for (int i = take + rank * kPickThreads + tid; i < p.s.n_pages; i += ranks * kPickThreads) to[i] = -1;
+    for (int i = take + rank * THREADS + tid; i < p.s.n_pages; i += ranks * THREADS) to[i] = -1;
     if (pages <= p.s.n_pages) {
-        for (int i = rank * kPickThreads + tid; i < pages; i += ranks * kPickThreads) to[i] = i;
+        for (int i = rank * THREADS + tid; i < pages; i += ranks * THREADS) to[i] = i;
         return;  // the whole row
     }
     const int slice = ((pages + ranks - 1) / ranks + 31) / 32 * 32;
@@ -379,22 +378,22 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     const int max_tiles = (v.table_pages + 15) / 16;
     uint32_t top = tid < (pages + 15) / 16 ? p.tops[(size_t)bh * max_tiles + tid] : 0;
     if (!p.spill) {
-        for (int i = tid; i < m; i += 8 * kPickThreads) {
+        for (int i = tid; i < m; i += 8 * THREADS) {
             uint32_t x[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = keys[min(i + j * kPickThreads, m - 1)];
+            for (int j = 0; j < 8; ++j) x[j] = keys[min(i + j * THREADS, m - 1)];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (i + j * kPickThreads < m) slice_keys[i + j * kPickThreads] = x[j];
+                if (i + j * THREADS < m) slice_keys[i + j * THREADS] = x[j];
         }
         keys = slice_keys;
     }
-    for (int i = tid + kPickThreads; i < (pages + 15) / 16; i += kPickThreads) top = max(top, p.tops[(size_t)bh * max_tiles + i]);
+    for (int i = tid + THREADS; i < (pages + 15) / 16; i += THREADS) top = max(top, p.tops[(size_t)bh * max_tiles + i]);
     top = __reduce_max_sync(~0u, top);
     if (lane == 0) warp_top[warp] = top;
     __syncthreads();
-    top = __reduce_max_sync(~0u, lane < kPickWarps ? warp_top[lane] : 0u);
-    const Cut<uint32_t> cut = row_cut<uint32_t, kPickThreads, LONE>(keys, m, take, kTaken32, cut_shared.approx);
+    top = __reduce_max_sync(~0u, lane < kWarps ? warp_top[lane] : 0u);
+    const Cut<uint32_t> cut = row_cut<uint32_t, THREADS, LONE>(keys, m, take, kTaken32, cut_shared.approx);
 
     // Pages above `in` are taken and pages below `out` are not, whatever the
     // error; without a finite one (infinities, NaN) every page is in question.
@@ -413,7 +412,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         if (cut.lo > kKeyMinusInf) out = key32_of(low - 2.f * error - fabsf(low) * 0x1p-22f);
     }
     // A warp's run of the slice, in page order.
-    const int run = ((m + kPickWarps - 1) / kPickWarps + 31) / 32 * 32;
+    const int run = ((m + kWarps - 1) / kWarps + 31) / 32 * 32;
     const int i0 = min(m, warp * run), i1 = min(m, i0 + run);
     const uint32_t below = (1u << lane) - 1;
     int above = 0, at_cut = 0, above_all, cut_all;
@@ -422,8 +421,8 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         above += __popc(__ballot_sync(~0u, k > in));
         at_cut += __popc(__ballot_sync(~0u, k >= out && k <= in));
     }
-    int above_at = warps_before<kPickThreads>(above, slots, &above_all);
-    int cut_at = warps_before<kPickThreads>(at_cut, slots, &cut_all);
+    int above_at = warps_before<THREADS>(above, slots, &above_all);
+    int cut_at = warps_before<THREADS>(at_cut, slots, &cut_all);
     const int2 before = row_before<LONE>(make_int2(above_all, cut_all), rank_slots[0]);
     above_at += before.x;
     cut_at += before.y;
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
             at += __popc(mask);
         }
         __syncthreads();
-        for (int i = before.y + warp; i < before.y + cut_all; i += kPickWarps) {
+        for (int i = before.y + warp; i < before.y + cut_all; i += kWarps) {
             const int lp = close_page[i], page = table[lp].x;
             const uint64_t key = page < 0 || page >= v.pool_pages ? 1 : exact_key<F16, D>(p, h, page, queries);
             if (lane < ranks) {
@@ -464,7 +463,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         }
         row_sync<LONE>();
         // keys at the cut become 0 (left out) or kTaken32.
-        for (int i = tid; i < row_close; i += kPickThreads) {
+        for (int i = tid; i < row_close; i += THREADS) {
             const Close mine = close[i];
             int better = 0;
             for (int j = 0; j < row_close; ++j)
@@ -494,12 +493,12 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
         if (lane == 0) exact[i] = key;
     }
     __syncthreads();
-    const Cut<uint64_t> fine = row_cut<uint64_t, kPickThreads, LONE>(exact, m, take, kTaken, cut_shared.exact);
+    const Cut<uint64_t> fine = row_cut<uint64_t, THREADS, LONE>(exact, m, take, kTaken, cut_shared.exact);
     int equal = 0;  // keys of the cut's range before this run
     if (fine.partial) {
         int mine = 0, all;
         for (int i = i0 + lane; i < i1; i += 32) mine += exact[i] >= fine.lo && exact[i] <= fine.hi;
-        equal = warps_before<kPickThreads>(__reduce_add_sync(~0u, mine), slots, &all);
+        equal = warps_before<THREADS>(__reduce_add_sync(~0u, mine), slots, &all);
         equal += row_before<LONE>(make_int2(all, 0), rank_slots[1]).x;
     }
     auto kept_mask = [&](int i, int* seen_equal) {
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(kPickThreads) page_pick_kernel(const SelectPar
     };
     int count = 0, at = equal, all;
     for (int i = i0; i < i1; i += 32) count += __popc(kept_mask(i + lane, &at));
-    int place = warps_before<kPickThreads>(count, slots, &all);
+    int place = warps_before<THREADS>(count, slots, &all);
     place += row_before<LONE>(make_int2(all, 0), rank_slots[2]).x;
     at = equal;
     for (int i = i0; i < i1; i += 32) {
@@ -543,7 +542,7 @@ struct LaunchBounds {
     }
 };
 struct SelectSpace {
-    int cluster;
+    int cluster, threads;
     bool spill;
     size_t slice, tops, all;
 };
@@ -555,6 +554,10 @@ SelectSpace select_space(const BatchView& v) {
     while (s.cluster < kMaxCluster && (pages + s.cluster - 1) / s.cluster > kMaxSlice) s.cluster *= 2;
     s.slice = ((pages + s.cluster - 1) / s.cluster + 31) / 32 * 32;
     s.spill = s.slice > kMaxSlice;
+    // Barriers of 32 warps against passes over more keys a thread: a step over
+    // 2049 pages took 25.3 us with 512 threads and 26.3 with 1024, one over up to
+    // 6035 pages 54.0 and 50.5.
+    s.threads = s.slice > 4096 ? 1024 : 512;
     const size_t approx = rows * pages * sizeof(uint64_t);
     s.tops = approx + rows * pages * sizeof(uint32_t);
     s.all = s.tops + rows * ((pages + 15) / 16) * sizeof(uint32_t);
@@ -575,8 +578,10 @@ struct LaunchSelect {
         cudaError_t e = p.group > 8 ? launch_dependent(page_score_kernel<F16, D, 2>, grid, block, base, stream, q)
                                     : launch_dependent(page_score_kernel<F16, D, 1>, grid, block, base, stream, q);
         if (e != cudaSuccess) return e;
-        return launch_cluster(s.cluster == 1 ? page_pick_kernel<F16, D, true> : page_pick_kernel<F16, D, false>,
-                              (unsigned)(p.v.batch * p.v.hkv), s.cluster, kPickThreads,
+        auto* pick = s.cluster > 1 ? page_pick_kernel<F16, D, false, 1024>
+                     : s.threads == 1024 ? page_pick_kernel<F16, D, true, 1024>
+                                         : page_pick_kernel<F16, D, true, 512>;
+        return launch_cluster(pick, (unsigned)(p.v.batch * p.v.hkv), s.cluster, s.threads,
                               sizeof(float) * p.group * D + (s.spill ? 0 : s.slice * sizeof(uint32_t)), stream, q);
     }
 };
@@ -584,8 +589,9 @@ struct ConfigureSelect {
     template <bool F16, int D>
     cudaError_t operator()() const {
         constexpr size_t kMost = kMaxSlice * sizeof(uint32_t) + sizeof(float) * kMaxBatchGroup * D;
-        const cudaError_t e = configure_kernel(page_pick_kernel<F16, D, true>, kMost);
-        return e != cudaSuccess ? e : configure_kernel(page_pick_kernel<F16, D, false>, kMost);
+        cudaError_t e = configure_kernel(page_pick_kernel<F16, D, true, 512>, kMost);
+        if (e == cudaSuccess) e = configure_kernel(page_pick_kernel<F16, D, true, 1024>, kMost);
+        return e != cudaSuccess ? e : configure_kernel(page_pick_kernel<F16, D, false, 1024>, kMost);
     }
 };
 

@@ -6,7 +6,7 @@
 // and summed over the cluster through distributed shared memory; the bucket
 // the cut falls into becomes the next range. Starting from the keys' own
 // smallest and largest values, a spread row is cut in one to three passes, any
-// row in ceil(bits / BITS). A lone CTA takes 2048 buckets; in a cluster 512, as
+// row in ceil(bits / BITS). A lone CTA takes 2048 buckets; in a cluster one a thread, as
 // each CTA reads every rank's counts and 2048 of them took longer than the pass
 // they save.
 #pragma once
@@ -39,7 +39,7 @@ __device__ __forceinline__ T* at_rank(T* p, int r) {
 
 template <typename K, int THREADS, bool LONE>
 struct CutShared {
-    static constexpr int kBits = LONE ? 11 : 9, kBins = 1 << kBits;
+    static constexpr int kBits = LONE ? 11 : THREADS > 512 ? 10 : 9, kBins = 1 << kBits;
     int hist[2][kBins];
     K range[2];       // this CTA's smallest and largest undecided key
     int2 counts;      // how many keys it takes first, and how many others it has

@@ -521,7 +521,7 @@ typedef struct gkv_batch_decode_args {
     const void* k_new;       /* [batch][Hkv][D] this step's token, or both NULL: attend only */
     const void* v_new;
     int64_t k_stride_batch, k_stride_head, v_stride_batch, v_stride_head;
-    void* out;               /* [batch][Hq][D] contiguous */
+    void* out;               /* [batch][Hq][D] contiguous, apart from every input */
     float* lse;              /* [batch][Hq] natural log of the sum of exponentials, or NULL */
     const int32_t* pages;    /* [batch][Hkv][n_pages] logical pages to attend, or NULL: all */
     const float* weights_in; /* [batch][Hkv][weights_stride], or NULL: zeros */
