@@ -199,3 +199,49 @@ def test_managed_prompt_then_sparse_steps():
     dense = BatchDecode(cache, c.q, c.k_new, c.v_new)
     ref.check_close(dense.run(), want["out"], want["slack"])
     assert cache.check_device_errors() == 0
+
+
+def test_a_managed_layer_evicted_and_decoded_on():
+    """A manager's layer cut back by the batch operators, its freed pages back
+    in the pool, then more tokens through the manager's own decode."""
+    from genllm_b200.batch import BatchDecode, CacheEvict, PagedBatch
+    from genllm_b200.paged_attention import PagedAttentionManager, paged_attention
+    g = torch.Generator("cuda").manual_seed(4)
+    hq, hkv, d, prompt, keep = 16, 8, 128, 500, 100
+    randn = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    m = PagedAttentionManager(0)
+    m.init_layer(0, hkv, d)
+    m.reserve_layer(0, 40)
+    paged_attention(m, 0, randn(1, hq, prompt, d), randn(1, hkv, prompt, d), randn(1, hkv, prompt, d))
+    k_ids, v_ids = m.page_table(0)
+    k_pool, v_pool = m.pool_tensors(0)
+    table = torch.tensor([list(zip(k_ids, v_ids))], dtype=torch.int32, device="cuda")
+    c = ref.Case(k_pool, v_pool, table, torch.tensor([prompt], dtype=torch.int32, device="cuda"), randn(1, hq, d),
+                 randn(1, hkv, d), randn(1, hkv, d))
+    cache = PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+    weights = torch.zeros(1, hkv, 16 * table.shape[1], device="cuda")
+    for _ in range(5):  # totals over the cached tokens alone
+        c.q.copy_(randn(1, hq, d))
+        BatchDecode(cache, c.q, weights=weights, weights_out=weights).run()
+    want = ref.evict(c, weights, c.lens.clone(), keep, 20)
+    CacheEvict(cache, weights, c.lens.clone(), keep=keep, recent=20, lens_out=c.lens).run()
+    left = -(-keep // 16)
+    m.set_page_table(0, k_ids[:left], v_ids[:left], keep)
+    for which, ids in ((0, k_ids), (1, v_ids)):
+        for i in reversed(ids[left:]):
+            m.pool(0, which).free(i)
+    assert same(c.k_pool, want[3]) and same(c.v_pool, want[4])
+    for step in range(20):
+        q, k, v = randn(1, hq, 1, d), randn(1, hkv, 1, d), randn(1, hkv, 1, d)
+        n = m.get_layer(0).num_cached
+        ids = m.page_table(0)
+        c.table = torch.tensor([list(zip(*ids))], dtype=torch.int32, device="cuda")
+        c.lens.fill_(n)
+        c.q, c.k_new, c.v_new = q[:, :, 0], k[:, :, 0], v[:, :, 0]
+        expect = ref.decode(c)
+        out = paged_attention(m, 0, q, k, v)
+        torch.cuda.synchronize()
+        err = (out[0, :, 0].double() - expect["out"][0]).abs()
+        # the op's own bounds: 2e-3 absolute, and one rounding to bf16
+        assert float((err - 2 ** -8 * expect["out"][0].abs()).max()) <= 2e-3, step
+    assert m.get_layer(0).num_cached == keep + 20 and m.check_device_errors(0) == 0
