@@ -81,6 +81,18 @@ def test_select_ties_nan_and_forced_pages():
     assert 15 in select_pages(cache, c.q, bound, 2, first=0, last=0, extra=0)[0, 1].tolist()
 
 
+def test_bounds_of_forced_pages_are_not_looked_at():
+    from genllm_b200.batch import page_bounds, select_pages
+    c = ref.make_case([700, 90], 8, 4, 128, torch.bfloat16, seed=9)
+    cache = cache_of(c)
+    bound = page_bounds(cache)
+    want = ref.select(c, bound, 6, 2, 1, 1)
+    for b, n in ((0, 700), (1, 90)):
+        for lp in (0, 1, n // 16):
+            bound[int(c.table[b, lp, 0])] = float("nan") if b else float("inf")
+    assert torch.equal(select_pages(cache, c.q, bound, 6, first=2, last=1, extra=1).cpu(), want)
+
+
 def test_select_zero_queries():
     """All scores equal: the lowest pages."""
     from genllm_b200.batch import page_bounds, select_pages
