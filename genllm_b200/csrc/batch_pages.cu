@@ -10,6 +10,8 @@
 // summed again in fp64 (in which products of 16-bit floats are exact). On 213
 // thousand tokens of 8 sequences, 8 kv heads of 128 (54 MB of bounds, 8 us), the
 // scores take 15 us and the cut 15; all pages in fp64 had taken 87.
+#include <algorithm>
+
 #include "batch.cuh"
 #include "cut.cuh"
 
@@ -540,7 +542,13 @@ struct LaunchBounds {
     cudaStream_t stream;
     template <bool F16, int D>
     cudaError_t operator()() const {
-        return launch_dependent(page_bounds_kernel<F16, D>, dim3(p.v.sms * kBoundsCtas), dim3(kBoundsThreads),
+        // From a start on, the pages of a step or a chunk: a CTA per SM, so that the
+        // kernel behind finds room beside them (a sparse step of 32k tokens waited
+        // 1.5 us for four). From 0 on, all the SMs hold.
+        const int64_t per_page = (int64_t)p.v.hkv * (D / 8) * 2, pages = p.start ? 4 : p.v.table_pages;
+        const int64_t most = (p.v.batch * pages * per_page + kBoundsThreads - 1) / kBoundsThreads;
+        const int64_t ctas = std::min<int64_t>(p.start ? std::max<int64_t>(most, p.v.sms) : most, p.v.sms * kBoundsCtas);
+        return launch_dependent(page_bounds_kernel<F16, D>, dim3((unsigned)ctas), dim3(kBoundsThreads),
                                 sizeof(int) * (size_t)(p.v.batch + 1), stream, p);
     }
 };
