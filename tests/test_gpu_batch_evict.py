@@ -245,3 +245,78 @@ def test_a_managed_layer_evicted_and_decoded_on():
         # the op's own bounds: 2e-3 absolute, and one rounding to bf16
         assert float((err - 2 ** -8 * expect["out"][0].abs()).max()) <= 2e-3, step
     assert m.get_layer(0).num_cached == keep + 20 and m.check_device_errors(0) == 0
+
+
+def test_batch_and_managed_steps_in_turn_without_waiting():
+    """A token through the batch decode, the next through the manager's own
+    decode, which streams pages ahead of its predecessor's end: each sees what
+    the other wrote, with the host waiting for neither."""
+    from genllm_b200.batch import BatchDecode, PagedBatch
+    from genllm_b200.paged_attention import PagedAttentionManager, paged_attention
+    g = torch.Generator("cuda").manual_seed(5)
+    hq, hkv, d, prompt, steps = 16, 8, 128, 1000, 60
+    randn = lambda *s: torch.randn(s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    m = PagedAttentionManager(0)
+    m.init_layer(0, hkv, d)
+    m.reserve_layer(0, 80)
+    K, V = randn(1, hkv, prompt, d), randn(1, hkv, prompt, d)
+    paged_attention(m, 0, randn(1, hq, prompt, d), K, V)
+    new = [(randn(1, hq, 1, d), randn(1, hkv, 1, d), randn(1, hkv, 1, d)) for _ in range(steps)]
+    k_pool, v_pool = m.pool_tensors(0)
+    table = torch.zeros(1, 80, 2, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([prompt], dtype=torch.int32, device="cuda")
+    cache = PagedBatch(k_pool, v_pool, table, lens)
+    outs, ops = [], []
+    torch.cuda.synchronize()
+    for i, (q, k, v) in enumerate(new):
+        if i % 2:
+            outs.append(paged_attention(m, 0, q, k, v)[0, :, 0])
+        else:
+            m.append_kv_pages(0, 1)  # the host's count; the batch decode writes the row
+            ids = torch.tensor(list(zip(*m.page_table(0))), dtype=torch.int32)
+            table[0, :len(ids)].copy_(ids.pin_memory(), non_blocking=True)
+            ops.append(BatchDecode(cache, q[:, :, 0], k[:, :, 0], v[:, :, 0]))
+            outs.append(ops[-1].run()[0])
+        lens += 1
+    torch.cuda.synchronize()
+    keys = torch.cat([K[0]] + [k[0] for _, k, _ in new], 1).double()
+    values = torch.cat([V[0]] + [v[0] for _, _, v in new], 1).double()
+    for i, (q, _, _) in enumerate(new):
+        n = prompt + i + 1
+        s = torch.einsum("hgd,hnd->hgn", q[0, :, 0].double().view(hkv, 2, d), keys[:, :n]) * d ** -0.5
+        want = (s.softmax(-1) @ values[:, :n]).reshape(hq, d)
+        err = (outs[i].double() - want).abs() - 2 ** -8 * want.abs()
+        assert float(err.max()) <= 2e-3, i  # the decode op's own bound beside one rounding
+    assert cache.check_device_errors() == 0 and m.check_device_errors(0) == 0
+
+
+def test_two_operators_in_one_captured_step():
+    """Two layers' decodes and an eviction in one graph, replayed between eager calls of the same operators."""
+    from genllm_b200.batch import BatchDecode, CacheEvict, PagedBatch
+    cases = [ref.make_case([90, 200], 8, 4, 64, torch.bfloat16, seed=40 + i, spare=40) for i in range(2)]
+    caches = [PagedBatch(c.k_pool, c.v_pool, c.table, c.lens) for c in cases]
+    steps = [BatchDecode(x, c.q, c.k_new, c.v_new) for x, c in zip(caches, cases)]
+    w = torch.rand((2, 4, 16 * cases[1].table.shape[1]), device="cuda")
+    cut = CacheEvict(caches[1], w, cases[1].lens.clone(), keep=60, recent=4, positions_out=torch.zeros(w.shape, dtype=torch.int32, device="cuda"))
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        for s in steps:
+            s.run()
+    for i in range(6):
+        wants = [ref.decode(c) for c in cases]
+        if i % 2:
+            for s in steps:
+                s.run()
+        else:
+            graph.replay()
+        for s, want in zip(steps, wants):
+            ref.check_close(s.out, want["out"], want["slack"])
+        for c in cases:
+            c.lens += 1
+        if i == 3:
+            want = ref.evict(cases[1], w, cases[1].lens.clone(), 60, 4)
+            CacheEvict(caches[1], w, cases[1].lens.clone(), keep=60, recent=4, lens_out=cases[1].lens).run()
+            assert same(cases[1].k_pool, want[3]) and torch.equal(cases[1].lens, want[0])
+    del cut
