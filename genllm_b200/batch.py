@@ -177,6 +177,8 @@ class BatchDecode(_Bound):
         _expect(out, "out", dev, out.dtype, (b, hq, d))
         if lse is True:
             lse = torch.empty((b, hq), dtype=torch.float32, device=dev)
+        elif lse is False:
+            lse = None
         if lse is not None:
             _expect(lse, "lse", dev, torch.float32, (b, hq))
         if pages is not None:

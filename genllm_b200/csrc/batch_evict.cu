@@ -30,7 +30,7 @@ struct EvictParams {
     BatchView v;
     EvictLaunch e;
     int32_t* counts;   // [batch * hkv] moves of each head
-    int32_t* left;     // [batch] new length, -1: skipped
+    int32_t* left;     // [batch] new length, below 0: skipped
     Move* moves;       // [batch * hkv][8 * table_pages]: a head moves at most half its slots
     uint32_t* keys;    // [batch * hkv][16 * table_pages] where a slice does not fit in shared memory; else null
 };
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     if (len > cap && first) atomicOr(v.err, kErrBadLength);
     const int n = min(len, cap), left = min(n, p.e.n_keep);
     if (first) {
-        if (bh % v.hkv == 0) p.left[b] = len < 0 ? -1 : left;
+        if (bh % v.hkv == 0) p.left[b] = len < 0 ? len : left;
         if (n <= left || left == 0) p.counts[bh] = 0;
     }
     if (len < 0 || left == 0) return;  // the whole cluster
@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
     const int lane = threadIdx.x & 31;
     const int bh = blockIdx.y, b = bh / v.hkv, h = bh % v.hkv;
     const int left = p.left[b], count = p.counts[bh];
-    if (left < 0) return;
     if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) p.e.lens_out[b] = left;
+    if (left < 0) return;
     const Move* moves = p.moves + (size_t)bh * v.table_pages * (kPageSlots / 2);
     const int2* table = v.table + b * v.table_stride;
     const int step = gridDim.x * (kMoveThreads / 32) * kGroup;

@@ -28,7 +28,7 @@ def check(c, w, seen, keep, recent, tracked=None, positions=None, in_place=False
         options = dict(lens_out=c.lens)
     else:
         first_positions = positions if positions is not None else torch.zeros(w.shape, dtype=torch.int32, device="cuda")
-        options = dict(weights_out=w.clone(), positions_out=first_positions.clone(), lens_out=c.lens.clone())
+        options = dict(weights_out=w.clone(), positions_out=first_positions.clone())
     old = w.clone()
     op = CacheEvict(cache, w, seen, keep=keep, recent=recent, tracked=tracked, positions=positions, **options)
     lens = op.run()
