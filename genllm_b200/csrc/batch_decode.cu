@@ -830,8 +830,9 @@ DecodeSpace decode_space(const BatchView& v, const BatchSplit& s, int n_q_heads,
 BatchSplit batch_split(const BatchView& v) {
     BatchSplit s;
     s.warps = v.dim == 256 ? 4 : 8;
-    s.heads = v.hkv < s.warps ? v.hkv : s.warps;
-    s.groups = (v.hkv + s.heads - 1) / s.heads;
+    // Groups of like size, so that a unit costs the same in each.
+    s.groups = (v.hkv + s.warps - 1) / s.warps;
+    s.heads = (v.hkv + s.groups - 1) / s.groups;
     s.lanes = s.warps / s.heads;
     s.grid = v.sms < kMaxGrid ? v.sms : kMaxGrid;
     s.workers = s.grid * s.lanes;

@@ -634,8 +634,8 @@ cudaError_t launch_select_pages(const BatchView& v, const SelectLaunch& s, cudaS
     p.v = v;
     p.s = s;
     p.group = s.n_q_heads / v.hkv;
-    p.heads = v.hkv < kScoreWarps ? v.hkv : kScoreWarps;
-    p.groups = (v.hkv + p.heads - 1) / p.heads;
+    p.groups = (v.hkv + kScoreWarps - 1) / kScoreWarps;
+    p.heads = (v.hkv + p.groups - 1) / p.groups;
     p.lanes = kScoreWarps / p.heads;
     p.workers = 0;
     p.exact = reinterpret_cast<uint64_t*>(w);
