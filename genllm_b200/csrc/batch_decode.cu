@@ -518,13 +518,14 @@ __device__ __forceinline__ void store_lse(const DecodeParams& p, size_t q_row, f
 }
 
 // Joins the parts of each cut sequence, in order. A segment of at most 32
-// parts is joined one row (query head) a warp, a longer one one row a CTA; when
-// these are few (one long sequence), a quarter of a row's dims a CTA, so that
-// its parts (2.4 MB at 32 heads and 147 parts) are fetched by many SMs. Bound:
-// latency. Everything but the loads comes before the wait for the decode
-// kernel, no load depends on another, and each maximum and sum is loaded once a
-// CTA: once a warp took 4000 cycles, all of them asking the same few lines of
-// L2. 72 registers, so that a CTA fits beside one of the decode kernel.
+// parts is joined one row (query head) a warp, a longer one by two to eight
+// warps a row; when these are few (one long sequence), a quarter of a row's dims
+// a CTA, so that its parts (2.4 MB at 32 heads and 147 parts) are fetched by
+// many SMs. Bound: latency (2 us behind the wait). Everything but the loads
+// comes before the wait for the decode kernel, no load depends on another, and
+// a CTA of one row loads each maximum and sum once: once a warp took 4000 cycles
+// at 147 parts, all of them asking the same few lines of L2. 72 registers, so
+// that a CTA fits beside one of the decode kernel.
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kJoinCuts = 4, kFewParts = 32;
 constexpr int kMaxParts = kMaxGrid * 8;
 
@@ -538,7 +539,7 @@ struct JoinShared {
 
 // One row's dims [cut * D / CUTS, + D / CUTS) from its `parts` parts, by the CTA.
 template <int D, int CUTS, typename Slot>
-__device__ __forceinline__ void join_many(const DecodeParams& p, JoinShared& sh, int parts, Slot slot, size_t q_row, int cut) {
+__device__ __forceinline__ void join_row(const DecodeParams& p, JoinShared& sh, int parts, Slot slot, size_t q_row, int cut) {
     constexpr int kSpan = D / CUTS, kLanes = kSpan / 4 < 32 ? kSpan / 4 : 32;  // lanes of a part's span
     constexpr int kVecs = kSpan / 4 / kLanes;          // 16-byte loads of a lane and part
     constexpr int kStep = kJoinWarps * (32 / kLanes);  // parts of the CTA's one load
@@ -553,12 +554,12 @@ __device__ __forceinline__ void join_many(const DecodeParams& p, JoinShared& sh,
 #pragma unroll
             for (int j = 0; j < kVecs; ++j) {
                 const int i = from + k * kStep;
-                x[k][j] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * D + dims + j * kLanes * 4)
+                x[k][j] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot(i) * D + dims + j * kLanes * 4))
                                     : make_float4(0.f, 0.f, 0.f, 0.f);
             }
     };
     load(part0);
-    for (int i = threadIdx.x; i < parts; i += kJoinThreads) sh.ml[i] = p.part_ml[slot(i)];
+    for (int i = threadIdx.x; i < parts; i += kJoinThreads) sh.ml[i] = __ldcg(&p.part_ml[slot(i)]);
     __syncthreads();
     float m = -INFINITY;
     for (int i = lane; i < parts; i += 32) m = fmaxf(m, sh.ml[i].x);
@@ -610,12 +611,108 @@ __device__ __forceinline__ void join_many(const DecodeParams& p, JoinShared& sh,
     __syncthreads();
 }
 
+// One row by WARPS of the CTA's warps, each finding the row's maximum and sum
+// for itself: several rows of a CTA, few warps asking the same lines. Every
+// thread of the CTA calls it (there: whether its row is one).
+template <int D, int WARPS, typename Slot>
+__device__ __forceinline__ void join_rows(const DecodeParams& p, JoinShared& sh, bool there, int parts, Slot slot,
+                                          size_t q_row) {
+    constexpr int kLanes = D / 4 < 32 ? D / 4 : 32;  // lanes of a part
+    constexpr int kVecs = D / 4 / kLanes;         // 16-byte loads of a lane and part
+    constexpr int kStep = WARPS * (32 / kLanes);  // parts of one load of the row's warps
+    constexpr int kBatch = 5;                     // parts of a lane in flight
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part0 = (warp % WARPS) * (32 / kLanes) + lane / kLanes;
+    const int dims = (lane % kLanes) * 4;
+    float m = -INFINITY, l = 0.f;
+    if (there) {
+        float4 x[kBatch][kVecs], acc[kVecs];
+        float top[kBatch];
+        auto load = [&](int from) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = from + k * kStep;
+                top[k] = i < parts ? __ldcg(&p.part_ml[slot(i)].x) : -INFINITY;
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j)
+                    x[k][j] = i < parts ? __ldcg(reinterpret_cast<const float4*>(p.part_acc + slot(i) * D + dims + j * kLanes * 4))
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        load(part0);
+        // A lane's running maximum and sum of parts lane, lane + 32, .., then the row's.
+        for (int i0 = 0; i0 < parts; i0 += 32 * kBatch) {
+            float2 ml[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * 32 + lane;
+                ml[k] = i < parts ? __ldcg(&p.part_ml[slot(i)]) : make_float2(-INFINITY, 0.f);
+            }
+            float n = m;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) n = fmaxf(n, ml[k].x);
+            l *= m == n ? 1.f : exp2_of(m - n);
+            m = n;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) l += ml[k].x == m ? ml[k].y : ml[k].y * exp2_of(ml[k].x - m);
+        }
+        const float mine = m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+        l *= mine == m ? 1.f : exp2_of(mine - m);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = part0;;) {
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const float f = i + k * kStep >= parts ? 0.f : top[k] == m ? 1.f : exp2_of(top[k] - m);
+#pragma unroll
+                for (int j = 0; j < kVecs; ++j) {
+                    acc[j].x += x[k][j].x * f;
+                    acc[j].y += x[k][j].y * f;
+                    acc[j].z += x[k][j].z * f;
+                    acc[j].w += x[k][j].w * f;
+                }
+            }
+            i += kBatch * kStep;
+            if (i - part0 >= parts) break;
+            load(i);
+        }
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+#pragma unroll
+            for (int o = kLanes; o < 32; o <<= 1) {
+                acc[j].x += __shfl_xor_sync(~0u, acc[j].x, o);
+                acc[j].y += __shfl_xor_sync(~0u, acc[j].y, o);
+                acc[j].z += __shfl_xor_sync(~0u, acc[j].z, o);
+                acc[j].w += __shfl_xor_sync(~0u, acc[j].w, o);
+            }
+            if (lane < kLanes) sh.acc[warp][j * kLanes + lane] = acc[j];
+        }
+    }
+    __syncthreads();
+    if (there) {
+        const float inv = m == -INFINITY ? 0.f : 1.f / l;  // no key at all: zeros
+        const int first = warp / WARPS * WARPS;
+        for (int d = (warp - first) * 32 + lane; d < D; d += WARPS * 32) {
+            float o = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) o += reinterpret_cast<const float*>(sh.acc[first + w])[d];
+            store_out(p.d.out, q_row * D + d, o * inv, p.d.out_dtype);
+        }
+        if (warp == first && lane == 0) store_lse(p, q_row, m, l);
+    }
+    __syncthreads();
+}
+
 // One row by a warp: lane i holds part i's factor.
 template <int D, typename Slot>
 __device__ __forceinline__ void join_few(const DecodeParams& p, int parts, Slot slot, size_t q_row) {
     constexpr int kPer = D / 32, kBatch = D == 256 ? 4 : 8;
     const int lane = threadIdx.x & 31;
-    const float2 ml = lane < parts ? p.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+    const float2 ml = lane < parts ? __ldcg(&p.part_ml[slot(lane)]) : make_float2(-INFINITY, 0.f);
     float2 x[kBatch][kPer / 2], acc[kPer / 2];
     auto load = [&](int from) {
 #pragma unroll
@@ -623,7 +720,7 @@ __device__ __forceinline__ void join_few(const DecodeParams& p, int parts, Slot 
 #pragma unroll
             for (int j = 0; j < kPer / 2; ++j)
                 x[k][j] = from + k < parts
-                              ? reinterpret_cast<const float2*>(p.part_acc + slot(from + k) * D + lane * kPer)[j]
+                              ? __ldcg(reinterpret_cast<const float2*>(p.part_acc + slot(from + k) * D + lane * kPer) + j)
                               : make_float2(0.f, 0.f);
     };
     load(0);
@@ -694,20 +791,26 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
         n_many += all >> 16;
     }
     __syncthreads();
+    // Of the longer segments' rows, as much to a CTA as leaves one item a CTA:
+    // a quarter of one, one, two or four.
     const int few_blocks = (rows + kJoinWarps - 1) / kJoinWarps;
-    const int cuts = n_many * rows * kJoinCuts <= (int)gridDim.x ? kJoinCuts : 1;
-    const int few_items = n_few * few_blocks, items = few_items + n_many * rows * cuts;
+    const int many_rows = n_many * rows, ctas = gridDim.x;
+    const int cuts = many_rows * kJoinCuts <= ctas ? kJoinCuts : 1;
+    const int together = many_rows <= ctas ? 1 : many_rows <= 2 * ctas ? 2 : 4;
+    const int few_items = n_few * few_blocks, items = few_items + (many_rows * cuts + together - 1) / together;
     bool waited = false;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    for (int item = blockIdx.x; item < items; item += ctas) {
         const bool few = item < few_items;
-        const int at = few ? item / few_blocks : (item - few_items) / (rows * cuts);
-        const int y = few ? item - at * few_blocks : item - few_items - at * rows * cuts;
-        const int seg = sh.cut_segs[few ? at : kMaxParts - 1 - at];
+        // A row of the CTA's warps: of its segment's, or of all the longer segments'.
+        const int line = few ? item / few_blocks : (item - few_items) / cuts * together + warp * together / kJoinWarps;
+        const int at = few ? line : line / rows;
+        const int row = few ? (item - at * few_blocks) * kJoinWarps + warp : line - at * rows;
+        const bool listed = few ? row < rows : line < many_rows;
+        const int seg = sh.cut_segs[few ? at : kMaxParts - 1 - (listed ? at : 0)];
         const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
         const int count = base[b + 1] - base[b];
         const int s0 = base[b] * p.s.groups + grp * count, w0 = s0 / per, parts = (s0 + count - 1) / per - w0 + 1;
-        const int row = few ? y * kJoinWarps + warp : y / cuts;
-        if (row >= rows || grp * p.s.heads + row / p.group >= p.v.hkv) continue;
+        const bool there = listed && grp * p.s.heads + row / p.group < p.v.hkv;
         // Part i lies in its worker's first slot, the segment's first part in the second unless it starts the worker's.
         const size_t slot0 = (size_t)2 * w0 * rows + row;
         const int shift0 = s0 != w0 * per ? rows : 0;
@@ -718,9 +821,17 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
             pdl_trigger();
             waited = true;
         }
-        if (few) join_few<D>(p, parts, slot, q_row);
-        else if (cuts == 1) join_many<D, 1>(p, sh, parts, slot, q_row, 0);
-        else join_many<D, kJoinCuts>(p, sh, parts, slot, q_row, y % cuts);
+        if (few) {
+            if (there) join_few<D>(p, parts, slot, q_row);
+        } else if (together == 1) {
+            // The CTA's warps have one row.
+            if (there && cuts > 1) join_row<D, kJoinCuts>(p, sh, parts, slot, q_row, (item - few_items) % cuts);
+            else if (there) join_row<D, 1>(p, sh, parts, slot, q_row, 0);
+        } else if (together == 2) {
+            join_rows<D, kJoinWarps / 2>(p, sh, there, parts, slot, q_row);
+        } else {
+            join_rows<D, kJoinWarps / 4>(p, sh, there, parts, slot, q_row);
+        }
     }
     // Every CTA waits, so that this kernel ends behind the decode kernel.
     if (!waited) {
@@ -733,12 +844,13 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
 // exp2(s_t - lse): a CTA per chunk of 1024 tokens of one (sequence, head), four
 // tokens a thread in flight. Bound: HBM and L2, 4 G + 8 bytes a token and head
 // (25 MB at 32768 tokens, 8 heads, G 4: 4.5 us of the step).
+template <int V>
+struct __align__(V * 4) Vec {
+    float x[V];
+};
 constexpr int kTotalsThreads = 256, kTotalsTokens = 4, kTotalsChunk = kTotalsThreads * kTotalsTokens;
 template <int V>  // scores of one load: the group is a multiple of it
 __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const DecodeParams p) {
-    struct __align__(V * 4) Vec {
-        float x[V];
-    };
     extern __shared__ int chunks[];
     __shared__ int warp_sums[32];
     const int G = p.group, hkv = p.v.hkv;
@@ -767,10 +879,10 @@ __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const Deco
             sum[i] = p.d.weights_in && t < min(n, len) ? p.d.decay * p.d.weights_in[row + t] : 0.f;
         }
         for (int g = 0; g < G; g += V) {
-            Vec x[kTotalsTokens];
+            Vec<V> x[kTotalsTokens];
 #pragma unroll
             for (int i = 0; i < kTotalsTokens; ++i)
-                x[i] = *reinterpret_cast<const Vec*>(s + (size_t)min(t0 + i * kTotalsThreads, units * kPageSlots - 1) * G + g);
+                x[i] = *reinterpret_cast<const Vec<V>*>(s + (size_t)min(t0 + i * kTotalsThreads, units * kPageSlots - 1) * G + g);
 #pragma unroll
             for (int i = 0; i < kTotalsTokens; ++i)
 #pragma unroll
