@@ -840,14 +840,15 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
     }
 }
 
-// weights_out[t] = decay * weights_in[t] + sum over the head's queries of
-// exp2(s_t - lse): a CTA per chunk of 1024 tokens of one (sequence, head), four
-// tokens a thread in flight. Bound: HBM and L2, 4 G + 8 bytes a token and head
-// (25 MB at 32768 tokens, 8 heads, G 4: 4.5 us of the step).
 template <int V>
 struct __align__(V * 4) Vec {
     float x[V];
 };
+
+// weights_out[t] = decay * weights_in[t] + sum over the head's queries of
+// exp2(s_t - lse): a CTA per chunk of 1024 tokens of one (sequence, head), four
+// tokens a thread in flight. Bound: HBM and L2, 4 G + 8 bytes a token and head
+// (25 MB at 32768 tokens, 8 heads, G 4: 4.5 us of the step).
 constexpr int kTotalsThreads = 256, kTotalsTokens = 4, kTotalsChunk = kTotalsThreads * kTotalsTokens;
 template <int V>  // scores of one load: the group is a multiple of it
 __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const DecodeParams p) {
