@@ -45,7 +45,7 @@ struct DecodeParams {
     float scale_log2;
     float* part_acc;     // [2 workers][heads * group][D]
     float2* part_ml;     // [2 workers][heads * group] (maximum in log2 units, sum)
-    float* lse2;         // [batch][Hq] log2 of the sum, for the totals
+    float* lse2;         // [batch][Hq] log2 of the sum, for the totals: -inf without a key, NaN if all scores were -inf
     float* scores;       // [unit][16][group] scores in log2 units, for the totals; or null
 };
 
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
                 if (whole) {
                     const float e = any_key ? m[nt][i] + log2f(l[nt][i]) : -INFINITY;
                     const size_t q_row = (size_t)b * hq + h * G + g;
-                    p.lse2[q_row] = e;
+                    p.lse2[q_row] = any_key && l[nt][i] == 0.f ? NAN : e;
                     if (p.d.lse) p.d.lse[q_row] = e * kLn2;
                 } else {
                     // A part whose scores were all -inf is told from one without keys by its maximum.
@@ -513,7 +513,7 @@ __device__ __forceinline__ int units_of(const DecodeParams& p, int b) {
 
 __device__ __forceinline__ void store_lse(const DecodeParams& p, size_t q_row, float m, float l) {
     const float e = m == -INFINITY ? -INFINITY : m + log2f(l);
-    p.lse2[q_row] = e;
+    p.lse2[q_row] = m != -INFINITY && l == 0.f ? NAN : e;
     if (p.d.lse) p.d.lse[q_row] = e * kLn2;
 }
 
@@ -887,7 +887,7 @@ __global__ void __launch_bounds__(kTotalsThreads) batch_totals_kernel(const Deco
 #pragma unroll
             for (int i = 0; i < kTotalsTokens; ++i)
 #pragma unroll
-                for (int k = 0; k < V; ++k) sum[i] += exp2_of(x[i].x[k] - e[g + k]);
+                for (int k = 0; k < V; ++k) sum[i] += e[g + k] == -INFINITY ? 0.f : exp2_of(x[i].x[k] - e[g + k]);
         }
 #pragma unroll
         for (int i = 0; i < kTotalsTokens; ++i) {

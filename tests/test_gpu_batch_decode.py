@@ -211,6 +211,24 @@ def test_bad_pages_and_lengths_are_flagged():
     assert torch.equal(pools.view(torch.int16), c.k_pool.view(torch.int16))
 
 
+@pytest.mark.parametrize("lens", [[40], [5000, 40]])
+def test_totals_of_a_sequence_of_bad_pages(lens):
+    """No page can be read: no attention, so the totals only decay."""
+    from genllm_b200.batch import PagedBatch, batch_decode
+    c = ref.make_case(lens, 8, 4, 64, torch.bfloat16, seed=17)
+    c.table[0] = -1
+    w = torch.rand(len(lens), 4, 16 * c.table.shape[1], device="cuda")
+    before = w.clone()
+    cache = PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+    lse = torch.zeros(len(lens), 8, device="cuda")
+    out = batch_decode(cache, c.q, c.k_new, c.v_new, lse=lse, weights=w, weights_out=w, decay=0.5)
+    assert cache.check_device_errors() == 1
+    n = lens[0]
+    assert bool((out[0] == 0).all()) and bool((lse[0] == -float("inf")).all())
+    assert torch.equal(w[0, :, :n], 0.5 * before[0, :, :n]) and bool((w[0, :, n] == 0).all())
+    assert torch.equal(w[0, :, n + 1:], before[0, :, n + 1:])
+
+
 def test_captured_steps_follow_the_lengths():
     """One capture, replayed while the lengths and the table move."""
     from genllm_b200.batch import PagedBatch, BatchDecode
