@@ -24,6 +24,7 @@ functions bind and run once. Every tensor lives on the pool's device.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional
 
 import torch
@@ -56,6 +57,17 @@ def _expect(t: torch.Tensor, what: str, device: torch.device, dtype, shape, cont
     if contiguous and not t.is_contiguous():
         raise _invalid(f"{what} must be contiguous")
     return t
+
+
+def _count(x, what: str) -> int:
+    """x as a 32-bit integer (the C structures would wrap a larger one around)."""
+    try:
+        n = operator.index(x)
+    except TypeError:
+        raise _invalid(f"{what} must be an integer, not {x!r}") from None
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise _invalid(f"{what} {n} is out of range")
+    return n
 
 
 def _rows(t: torch.Tensor, what: str, device: torch.device, dtype, shape) -> torch.Tensor:
@@ -220,7 +232,7 @@ class PageBounds(_Bound):
         self._hold(bounds, start)
         self.bounds = bounds
         self._bind(lib().gkv_batch_page_bounds, C.byref(cache.desc), start.data_ptr() if start is not None else None,
-                   int(extra), bounds.data_ptr(), result=bounds)
+                   _count(extra, "extra"), bounds.data_ptr(), result=bounds)
 
 
 class PageSelect(_Bound):
@@ -237,17 +249,18 @@ class PageSelect(_Bound):
         dev, b, hkv, d = cache.device, cache.batch, cache.n_kv_heads, cache.head_dim
         _rows(q, "q", dev, cache.dtype, (b, None, d))
         _expect(bounds, "bounds", dev, cache.dtype, (cache.pool_pages, hkv, 2, d))
+        n_pages = _count(n_pages, "n_pages")
+        first, last, extra = _count(first, "first"), _count(last, "last"), _count(extra, "extra")
         if n_pages < 1:
             raise _invalid(f"n_pages {n_pages}")
         if pages is None:
-            pages = torch.full((b, hkv, int(n_pages)), -1, dtype=torch.int32, device=dev)
-        _expect(pages, "pages", dev, torch.int32, (b, hkv, int(n_pages)))
+            pages = torch.full((b, hkv, n_pages), -1, dtype=torch.int32, device=dev)
+        _expect(pages, "pages", dev, torch.int32, (b, hkv, n_pages))
         size = C.c_size_t()
         check(lib().gkv_batch_select_workspace(C.byref(cache.desc), C.byref(size)))
         space = self._space(size.value)
         self.args = _lib.BatchSelectArgs(q.data_ptr(), q.stride(0), q.stride(1), bounds.data_ptr(), pages.data_ptr(),
-                                         int(n_pages), int(first), int(last), int(extra), q.shape[1],
-                                         space.data_ptr(), space.numel())
+                                         n_pages, first, last, extra, q.shape[1], space.data_ptr(), space.numel())
         self._hold(q, bounds, pages)
         self.pages = pages
         self._bind(lib().gkv_batch_select_pages, C.byref(cache.desc), C.byref(self.args), result=pages)
@@ -296,7 +309,7 @@ class CacheEvict(_Bound):
         ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
         self.args = _lib.BatchEvictArgs(weights.data_ptr(), weights_out.data_ptr(), ptr(positions),
                                         positions_out.data_ptr(), seen.data_ptr(), ptr(tracked), lens_out.data_ptr(),
-                                        shape[2], int(keep), int(recent), space.data_ptr(), space.numel())
+                                        shape[2], _count(keep, "keep"), _count(recent, "recent"), space.data_ptr(), space.numel())
         self._hold(weights, weights_out, positions, positions_out, seen, tracked, lens_out)
         self.lens_out, self.weights_out, self.positions_out = lens_out, weights_out, positions_out
         self._bind(lib().gkv_batch_evict, C.byref(cache.desc), C.byref(self.args), result=lens_out)

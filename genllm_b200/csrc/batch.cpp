@@ -124,6 +124,26 @@ int check_rows(const void* p, int64_t stride_batch, int64_t stride_head, const c
     return GKV_OK;
 }
 
+// Whether byte ranges [a, a + a_bytes) and [b, b + b_bytes) share a byte.
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y ? y - x < a_bytes : x - y < b_bytes;
+}
+
+// Bytes from the first to the last element of a strided [batch][heads][D]
+// tensor of 16-bit elements; 0 for strides that run backwards.
+size_t span_bytes(int64_t batch, int64_t heads, int64_t dim, int64_t stride_batch, int64_t stride_head) {
+    if (stride_batch < 0 || stride_head < 0) return 0;
+    return 2 * (size_t)((batch - 1) * stride_batch + (heads - 1) * stride_head + dim);
+}
+
+// An array and its successor: the same memory or apart.
+int check_successor(const void* in, const void* out, size_t bytes, const char* what) {
+    if (in && in != out && overlap(in, bytes, out, bytes))
+        return fail(GKV_ERR_INVALID, "%s overlaps its successor without being the same array", what);
+    return GKV_OK;
+}
+
 BatchView view_of(const gkv_batch* b, const DeviceState& s) {
     BatchView v;
     v.k_base = static_cast<uint16_t*>(b->pool.k_base);
@@ -215,9 +235,19 @@ int gkv_batch_decode(const gkv_batch* b, const gkv_batch_decode_args* a, gkv_str
             a->weights_stride < (int64_t)GKV_PAGE_SLOTS * b->table_pages)
             return fail(GKV_ERR_INVALID, "weights_stride %lld below 16 * table_pages", (long long)a->weights_stride);
         if (!std::isfinite(a->decay)) return fail(GKV_ERR_INVALID, "decay %g", (double)a->decay);
+        if (int st = check_successor(a->weights_in, a->weights_out,
+                                     sizeof(float) * (size_t)b->batch * b->pool.n_kv_heads * a->weights_stride, "weights_in"))
+            return st;
     } else if (a->weights_in) {
         return fail(GKV_ERR_INVALID, "weights_in without weights_out");
     }
+    // Rows of out are written while others' inputs are still read.
+    const int64_t n = b->batch, hkv = b->pool.n_kv_heads, dim = b->pool.head_dim;
+    const size_t out_bytes = (a->out_dtype == GKV_F32 ? 4 : 2) * (size_t)n * a->n_q_heads * dim;
+    if (overlap(a->out, out_bytes, a->q, span_bytes(n, a->n_q_heads, dim, a->q_stride_batch, a->q_stride_head)) ||
+        (a->k_new && (overlap(a->out, out_bytes, a->k_new, span_bytes(n, hkv, dim, a->k_stride_batch, a->k_stride_head)) ||
+                      overlap(a->out, out_bytes, a->v_new, span_bytes(n, hkv, dim, a->v_stride_batch, a->v_stride_head)))))
+        return fail(GKV_ERR_INVALID, "out overlaps an input");
     if (int st = check_space(a->workspace, a->workspace_bytes, 0)) return st;
     GKV_ENTER(b)
     const BatchView v = view_of(b, state);
@@ -314,6 +344,9 @@ int gkv_batch_evict(const gkv_batch* b, const gkv_batch_evict_args* a, gkv_strea
         if (!aligned(p, 4)) return fail(GKV_ERR_INVALID, "arrays must be 4-byte aligned");
     if (a->stride < (int64_t)GKV_PAGE_SLOTS * b->table_pages)
         return fail(GKV_ERR_INVALID, "stride %lld below 16 * table_pages", (long long)a->stride);
+    const size_t bytes = sizeof(float) * (size_t)b->batch * b->pool.n_kv_heads * a->stride;
+    if (int st = check_successor(a->weights, a->weights_out, bytes, "weights")) return st;
+    if (int st = check_successor(a->positions, a->positions_out, bytes, "positions")) return st;
     if (a->n_keep < 0 || a->n_recent < 0 || a->n_recent > a->n_keep)
         return fail(GKV_ERR_INVALID, "n_keep %d, n_recent %d", a->n_keep, a->n_recent);
     if ((int64_t)b->batch * b->pool.n_kv_heads > 65535)

@@ -521,11 +521,11 @@ typedef struct gkv_batch_decode_args {
     const void* k_new;       /* [batch][Hkv][D] this step's token, or both NULL: attend only */
     const void* v_new;
     int64_t k_stride_batch, k_stride_head, v_stride_batch, v_stride_head;
-    void* out;               /* [batch][Hq][D] contiguous, apart from every input */
+    void* out;               /* [batch][Hq][D] contiguous, apart from every input (refused otherwise) */
     float* lse;              /* [batch][Hq] natural log of the sum of exponentials, or NULL */
     const int32_t* pages;    /* [batch][Hkv][n_pages] logical pages to attend, or NULL: all */
     const float* weights_in; /* [batch][Hkv][weights_stride], or NULL: zeros */
-    float* weights_out;      /* the same shape, may be weights_in; NULL: no totals */
+    float* weights_out;      /* the same shape, weights_in itself or apart from it; NULL: no totals */
     int64_t weights_stride;  /* >= 16 * table_pages */
     int32_t n_pages;
     int32_t n_q_heads;
@@ -551,7 +551,8 @@ int gkv_batch_decode_workspace(const gkv_batch* b, int32_t n_q_heads, int32_t to
  * its page is listed. With weights_out (not together with `pages`):
  *   weights_out[b][h][t] = decay * weights_in[b][h][t] + sum over the query
  *   heads of h of the attention weight of token t
- * for every attended t; the new token's weights_in counts as 0. */
+ * for every attended t; the new token's weights_in counts as 0, and so does the
+ * attention of a token on a skipped page. */
 int gkv_batch_decode(const gkv_batch* b, const gkv_batch_decode_args* a, gkv_stream_t stream);
 
 /* bounds [pool_pages][Hkv][2][D] in the pool's dtype, indexed by K page id:
@@ -587,9 +588,9 @@ int gkv_batch_select_pages(const gkv_batch* b, const gkv_batch_select_args* a, g
 
 typedef struct gkv_batch_evict_args {
     const float* weights;      /* [batch][Hkv][stride] */
-    float* weights_out;        /* the same shape, may be `weights` */
+    float* weights_out;        /* the same shape, `weights` itself or apart from it */
     const int32_t* positions;  /* [batch][Hkv][stride], used below tracked[b]; NULL only with tracked NULL */
-    int32_t* positions_out;    /* the same shape, may be `positions` */
+    int32_t* positions_out;    /* the same shape, `positions` itself or apart from it */
     const int32_t* seen;       /* [batch] tokens the sequence has had in all: the next token's position */
     const int32_t* tracked;    /* [batch] slots whose position is in `positions`, or NULL: none */
     int32_t* lens_out;         /* [batch], may be lens */

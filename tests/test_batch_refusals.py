@@ -7,6 +7,7 @@ from genllm_b200 import _lib
 
 INVALID, UNSUPPORTED = _lib.GKV_ERR_INVALID, _lib.GKV_ERR_UNSUPPORTED
 ADDR = 1 << 20  # never read: every check comes first
+OUT = 1 << 24
 
 
 def batch(**changes):
@@ -18,7 +19,7 @@ def batch(**changes):
 
 
 def decode_args(**changes):
-    a = _lib.BatchDecodeArgs(ADDR, 1024, 128, ADDR, ADDR, 1024, 128, 1024, 128, ADDR, None, None, None, None, 0, 0, 16,
+    a = _lib.BatchDecodeArgs(ADDR, 1024, 128, ADDR, ADDR, 1024, 128, 1024, 128, OUT, None, None, None, None, 0, 0, 16,
                              _lib.GKV_BF16, 0.1, 1.0, ADDR, 0)
     for k, v in changes.items():
         setattr(a, k, v)
@@ -71,7 +72,10 @@ def test_batches(changes, status):
     (dict(pages=ADDR, n_pages=4, weights_out=ADDR, weights_stride=256), UNSUPPORTED),
     (dict(weights_in=ADDR), INVALID), (dict(weights_out=ADDR, weights_stride=255), INVALID),
     (dict(weights_out=ADDR, weights_stride=256, decay=float("inf")), INVALID), (dict(workspace=None), INVALID),
-    (dict(workspace=ADDR + 8), INVALID)])
+    (dict(workspace=ADDR + 8), INVALID), (dict(out=ADDR), INVALID),
+    (dict(q=OUT + 2 * 2 * 16 * 128 - 16), INVALID), (dict(q=OUT - 2 * (1024 + 16 * 128) + 16), INVALID),
+    (dict(k_new=OUT + 16), INVALID), (dict(v_new=OUT - 16), INVALID),
+    (dict(weights_in=ADDR, weights_out=ADDR + 4, weights_stride=256), INVALID)])
 def test_decode(changes, status):
     assert _lib.lib().gkv_batch_decode(C.byref(batch()), C.byref(decode_args(**changes)), None) == status
     assert _lib.lib().gkv_last_error()
@@ -92,9 +96,38 @@ def test_select(changes, status):
     (dict(seen=None), INVALID), (dict(lens_out=None), INVALID), (dict(tracked=ADDR), INVALID),
     (dict(weights=ADDR + 2), INVALID), (dict(stride=255), INVALID), (dict(n_keep=-1), INVALID),
     (dict(n_recent=-1), INVALID), (dict(n_recent=65), INVALID), (dict(workspace=None), INVALID),
-    (dict(workspace=ADDR + 4), INVALID)])
+    (dict(workspace=ADDR + 4), INVALID), (dict(weights_out=ADDR + 2 * 8 * 256 * 4 - 4), INVALID),
+    (dict(positions=ADDR + 4), INVALID)])
 def test_evict(changes, status):
     assert _lib.lib().gkv_batch_evict(C.byref(batch()), C.byref(evict_args(**changes)), None) == status
+
+
+def message(call, args):
+    """What the entry point says of arguments whose only fault is the empty workspace, or another one."""
+    assert call(C.byref(batch()), C.byref(args), None) != _lib.GKV_OK
+    return _lib.lib().gkv_last_error()
+
+
+def test_outputs_on_inputs_are_named():
+    L = _lib.lib()
+    assert b"out overlaps" in message(L.gkv_batch_decode, decode_args(out=ADDR, workspace=None))
+    assert b"workspace" in message(L.gkv_batch_decode, decode_args(workspace=None))
+    span = 2 * (1024 + 16 * 128)  # bytes of q with these strides
+    assert b"out overlaps" in message(L.gkv_batch_decode, decode_args(q=OUT - span + 16, workspace=None))
+    assert b"workspace" in message(L.gkv_batch_decode, decode_args(q=OUT - span, workspace=None))
+    assert b"workspace" in message(L.gkv_batch_decode, decode_args(
+        weights_in=ADDR, weights_out=ADDR, weights_stride=256, workspace=None))
+    end = ADDR + 2 * 8 * 256 * 4
+    assert b"workspace" in message(L.gkv_batch_evict, evict_args(weights_out=end, workspace=None))
+    assert b"successor" in message(L.gkv_batch_evict, evict_args(weights_out=end - 4, workspace=None))
+
+
+def test_counts_that_32_bits_do_not_hold():
+    from genllm_b200.batch import _count
+    assert _count(7, "keep") == 7 and _count(2 ** 31 - 1, "keep") == 2 ** 31 - 1
+    for bad in (2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1, 1.5, "3", None):
+        with pytest.raises(_lib.GkvError):
+            _count(bad, "keep")
 
 
 def test_bounds_and_nulls():
