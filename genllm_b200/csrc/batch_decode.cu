@@ -518,15 +518,15 @@ __device__ __forceinline__ void store_lse(const DecodeParams& p, size_t q_row, f
 }
 
 // Joins the parts of each cut sequence, in order. A segment of at most 32
-// parts is joined one row (query head) a warp, a longer one by two to eight
-// warps a row; when these are few (one long sequence), a quarter of a row's dims
+// parts is joined one row (query head) a warp, or by four if there is room, a
+// longer one by two to eight warps a row; when these are few (one long sequence), a quarter of a row's dims
 // a CTA, so that its parts (2.4 MB at 32 heads and 147 parts) are fetched by
 // many SMs. Bound: latency (2 us behind the wait). Everything but the loads
 // comes before the wait for the decode kernel, no load depends on another, and
 // a CTA of one row loads each maximum and sum once: once a warp took 4000 cycles
 // at 147 parts, all of them asking the same few lines of L2. 72 registers, so
 // that a CTA fits beside one of the decode kernel.
-constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kJoinCuts = 4, kFewParts = 32;
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32, kJoinCuts = 4, kFewParts = 32, kFetchParts = 8;
 constexpr int kMaxParts = kMaxGrid * 8;
 
 struct JoinShared {
@@ -766,7 +766,7 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
     const int total = base[p.v.batch] * p.s.groups;
     const int per = max(1, (total + p.s.workers - 1) / p.s.workers);
     // A cut segment belongs to the first boundary between workers inside it.
-    int n_few = 0, n_many = 0;
+    int n_few = 0, n_many = 0, n_some = 0;  // some: of the few, those that a warp does not fetch at once
     for (int w = 0; (int64_t)(w + 1) * per < total; w += kJoinThreads) {
         const int64_t u = (int64_t)(w + (int)threadIdx.x + 1) * per;  // the boundary's unit
         int seg = 0, parts = 0;
@@ -779,38 +779,47 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
         }
         const bool few = parts && parts <= kFewParts, many = parts > kFewParts;
         const uint32_t few_mask = __ballot_sync(~0u, few), many_mask = __ballot_sync(~0u, many);
+        const uint32_t some_mask = __ballot_sync(~0u, few && parts > kFetchParts);
         __syncthreads();
-        if (lane == 0) sh.slots[warp] = __popc(few_mask) | __popc(many_mask) << 16;
+        if (lane == 0) sh.slots[warp] = __popc(few_mask) | __popc(some_mask) << 10 | __popc(many_mask) << 20;
         __syncthreads();
         const int x = lane < kJoinWarps ? sh.slots[lane] : 0;
         const int before = __reduce_add_sync(~0u, lane < warp ? x : 0), all = __reduce_add_sync(~0u, x);
         const uint32_t below = (1u << lane) - 1;
-        if (few) sh.cut_segs[n_few + (before & 0xFFFF) + __popc(few_mask & below)] = seg;
-        if (many) sh.cut_segs[kMaxParts - 1 - (n_many + (before >> 16) + __popc(many_mask & below))] = seg;
-        n_few += all & 0xFFFF;
-        n_many += all >> 16;
+        if (few) sh.cut_segs[n_few + (before & 0x3FF) + __popc(few_mask & below)] = seg;
+        if (many) sh.cut_segs[kMaxParts - 1 - (n_many + (before >> 20) + __popc(many_mask & below))] = seg;
+        n_few += all & 0x3FF;
+        n_some += all >> 10 & 0x3FF;
+        n_many += all >> 20;
     }
     __syncthreads();
     // Of the longer segments' rows, as much to a CTA as leaves one item a CTA:
     // a quarter of one, one, two or four.
-    const int few_blocks = (rows + kJoinWarps - 1) / kJoinWarps;
-    const int many_rows = n_many * rows, ctas = gridDim.x;
+    const int many_rows = n_many * rows, few_rows = n_few * rows, ctas = gridDim.x;
     const int cuts = many_rows * kJoinCuts <= ctas ? kJoinCuts : 1;
     const int together = many_rows <= ctas ? 1 : many_rows <= 2 * ctas ? 2 : 4;
-    const int few_items = n_few * few_blocks, items = few_items + (many_rows * cuts + together - 1) / together;
+    const int many_items = (many_rows * cuts + together - 1) / together;
+    // The others' rows have a warp each, or, if that would fetch again and again
+    // and CTAs are left, four (8 sequences of 18 parts, 32 heads: 54.2 -> 51.1 us a
+    // sparse step; 5 of 24 to 340 pages, 40 heads: 15.6 -> 15.0).
+    const bool pairs = 2 * n_some > n_few && (few_rows + 1) / 2 + many_items <= ctas;
+    const int few_blocks = (rows + kJoinWarps - 1) / kJoinWarps;
+    const int few_items = pairs ? (few_rows + 1) / 2 : n_few * few_blocks, items = few_items + many_items;
     bool waited = false;
     for (int item = blockIdx.x; item < items; item += ctas) {
-        const bool few = item < few_items;
-        // A row of the CTA's warps: of its segment's, or of all the longer segments'.
-        const int line = few ? item / few_blocks : (item - few_items) / cuts * together + warp * together / kJoinWarps;
-        const int at = few ? line : line / rows;
-        const int row = few ? (item - at * few_blocks) * kJoinWarps + warp : line - at * rows;
-        const bool listed = few ? row < rows : line < many_rows;
-        const int seg = sh.cut_segs[few ? at : kMaxParts - 1 - (listed ? at : 0)];
+        const bool few = item < few_items, alone = few && !pairs;
+        // A row of the CTA's warps: of its segment's, or of all the list's.
+        const int line = alone ? item / few_blocks
+                         : few ? item * 2 + warp * 2 / kJoinWarps
+                               : (item - few_items) / cuts * together + warp * together / kJoinWarps;
+        const bool listed = alone || line < (few ? few_rows : many_rows);
+        const int at = !listed ? 0 : alone ? line : line / rows;
+        const int row = alone ? (item - at * few_blocks) * kJoinWarps + warp : line - at * rows;
+        const int seg = sh.cut_segs[few ? at : kMaxParts - 1 - at];
         const int b = seg / p.s.groups, grp = seg - b * p.s.groups;
         const int count = base[b + 1] - base[b];
         const int s0 = base[b] * p.s.groups + grp * count, w0 = s0 / per, parts = (s0 + count - 1) / per - w0 + 1;
-        const bool there = listed && grp * p.s.heads + row / p.group < p.v.hkv;
+        const bool there = listed && row < rows && grp * p.s.heads + row / p.group < p.v.hkv;
         // Part i lies in its worker's first slot, the segment's first part in the second unless it starts the worker's.
         const size_t slot0 = (size_t)2 * w0 * rows + row;
         const int shift0 = s0 != w0 * per ? rows : 0;
@@ -821,13 +830,13 @@ __global__ void __maxnreg__(72) batch_join_kernel(const DecodeParams p) {
             pdl_trigger();
             waited = true;
         }
-        if (few) {
+        if (alone) {
             if (there) join_few<D>(p, parts, slot, q_row);
-        } else if (together == 1) {
+        } else if (!few && together == 1) {
             // The CTA's warps have one row.
             if (there && cuts > 1) join_row<D, kJoinCuts>(p, sh, parts, slot, q_row, (item - few_items) % cuts);
             else if (there) join_row<D, 1>(p, sh, parts, slot, q_row, 0);
-        } else if (together == 2) {
+        } else if (few || together == 2) {
             join_rows<D, kJoinWarps / 2>(p, sh, there, parts, slot, q_row);
         } else {
             join_rows<D, kJoinWarps / 4>(p, sh, there, parts, slot, q_row);

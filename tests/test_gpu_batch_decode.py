@@ -173,6 +173,32 @@ def test_totals(hq, hkv, d, decay, in_place, append):
         ref.check_close(w_out[b, :, :m], exact, slack, f"totals of {n}")
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(8, 1, 64), (32, 2, 64), (14, 2, 128), (12, 3, 64), (20, 4, 128), (4, 1, 256), (32, 2, 256)])
+@pytest.mark.parametrize("lens", [[9000], [16 * 592], [16 * 1184 - 1], [300, 20000, 0, 15], [31, 5000, 47, 5000, 1],
+                                  [2000] * 9, [16 * 37] * 32])
+def test_workers_of_a_block_share_a_sequence(hq, hkv, d, lens):
+    """Few kv heads: several workers of a block hold parts of one sequence."""
+    c = ref.make_case(lens, hq, hkv, d, torch.bfloat16, seed=40)
+    out, lse = run(c)
+    check(c, out, lse, ref.decode(c))
+    again, lse_again = run(c)
+    assert torch.equal(out.view(torch.int16), again.view(torch.int16)) and torch.equal(lse, lse_again)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(8, 1, 64), (14, 2, 128), (20, 4, 128), (4, 1, 256)])
+def test_parts_without_a_key(hq, hkv, d):
+    """Lists of which long runs name no page: whole parts, and whole blocks' parts, attend nothing."""
+    c = ref.make_case([9000, 20000, 40], hq, hkv, d, torch.bfloat16, seed=41)
+    n = c.table.shape[1]
+    pages = torch.arange(n, dtype=torch.int32, device="cuda").expand(3, hkv, n).contiguous()
+    pages[0, :, :300] = -1
+    pages[1, 0, 20:1200] = -1
+    pages[1, hkv - 1, 700:] = -1
+    pages[2] = -1
+    out, lse = run(c, pages=pages)
+    check(c, out, lse, ref.decode(c, pages=pages))
+
+
 def test_totals_without_a_total_so_far():
     from genllm_b200.batch import PagedBatch, batch_decode
     c = ref.make_case([50], 4, 2, 64, torch.bfloat16)
