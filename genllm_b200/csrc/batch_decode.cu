@@ -140,6 +140,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
     constexpr int kCopies = kPageSlots / kRowsPerCopy;
     constexpr int kSteps = D / 16;
     constexpr int kTerms = F16 ? 2 : 3;  // of an attention weight
+    // f16 steps by 2^-24 at its bottom: weights (at most 1) are taken times 2^15, so
+    // that what two terms lose is 2^-40 of the part's largest, and not 2^-25. The
+    // sums (l) hold the weights as they are. bf16 reaches as far down as fp32.
+    constexpr float kLift = F16 ? 0x1p15f : 1.f;
     static_assert(kStages >= 2, "the ring holds one unit ahead");
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = raw_smem + (kRingAlign - smem_addr(raw_smem) % kRingAlign) % kRingAlign;
@@ -444,8 +448,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
                 const float p2 = exp2_of(s[nt][2] - m0), p3 = exp2_of(s[nt][3] - m1);
                 l[nt][0] += p0 + p2;
                 l[nt][1] += p1 + p3;
-                rest[nt][0] = make_float2(p0, p1);
-                rest[nt][1] = make_float2(p2, p3);
+                rest[nt][0] = make_float2(p0 * kLift, p1 * kLift);
+                rest[nt][1] = make_float2(p2 * kLift, p3 * kLift);
             }
             // The product with V takes P as a sum of 16-bit terms: three of bf16 hold all
             // 24 bits of a weight, two of f16 22. A third term is 0.5 % of a ragged step
@@ -475,7 +479,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[nt][i] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][i], o);
-                inv[i] = any_key ? 1.f / l[nt][i] : 0.f;
+                inv[i] = any_key ? 1.f / l[nt][i] / kLift : 0.f;
                 const int g = nt * 8 + c2 + i;
                 if (g4 != 0 || g >= G) continue;
                 if (whole) {
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) batch_decode_kernel(const Decod
             for (int i = 0; i < 2; ++i) {
                 const int g = nt * 8 + c2 + i;
                 if (g >= G) continue;
-                const float factor = whole ? inv[i] : 1.f;
+                const float factor = whole ? inv[i] : 1.f / kLift;
                 float* to = (whole ? static_cast<float*>(p.d.out) + ((size_t)b * hq + h * G) * D : p.part_acc + slot * D) +
                             (size_t)g * D + g4;
 #pragma unroll

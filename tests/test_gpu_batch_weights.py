@@ -45,6 +45,22 @@ def relative(gap, n):
     return (3 * gap + 4 + n + 8) * 2.0 ** -24
 
 
+@pytest.mark.parametrize("gap", [4.5, 11.75, 13.0, 16.0, 17.5])
+def test_small_weights_in_f16(gap):
+    """Whole sequences a worker, the leading token's value 0: the output is what
+    the weights far below the maximum hold. Of 2^15 times a weight two f16 terms
+    keep 22 bits, or steps of 2^-24: half a step is 2^-40 of the largest weight."""
+    from genllm_b200.batch import PagedBatch, batch_decode
+    n = 64
+    lens, gaps = [n] * 300, [gap] * 300
+    c = one_score_each(lens, gaps, torch.float16)
+    got = batch_decode(PagedBatch(c.k_pool, c.v_pool, c.table, c.lens), c.q, scale=1.0,
+                       out=torch.zeros(c.q.shape, device="cuda")).double()
+    want, sums = shares(c, gaps)
+    slack = want * (relative(gap, n) + 2.0 ** -22) + sums * 2.0 ** -40
+    assert float(((got - want).abs() - slack).max()) <= 0, float(((got - want).abs() / want).max())
+
+
 def test_weights_in_bf16_keep_their_bits():
     """An f32 output shows the weights' 24 bits: three bf16 terms hold them all."""
     from genllm_b200.batch import PagedBatch, batch_decode
