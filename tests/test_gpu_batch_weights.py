@@ -74,3 +74,26 @@ def test_weights_in_bf16_keep_their_bits():
     want, _ = shares(c, gaps)
     slack = want * torch.tensor([relative(gap, n) for gap in gaps], device="cuda").view(-1, 1, 1)
     assert float(((got - want).abs() - slack).max()) <= 0, float(((got - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hkv,group,d", [(1, 1, 64), (8, 4, 128), (2, 16, 256)])
+def test_every_page_of_a_long_row_is_in_the_output(hkv, group, d, dtype):
+    """Equal scores, page j's values 1 in dimension j mod D alone: an output is a
+    count over n, which holds one rounding of 1/n and one of the product."""
+    from genllm_b200.batch import PagedBatch, batch_decode
+    n = 30001
+    pages = -(-n // 16)
+    g = torch.Generator("cuda").manual_seed(2)
+    table = torch.stack([torch.randperm(pages, generator=g, device="cuda") for _ in range(2)], -1).int()[None].contiguous()
+    k_pool = torch.randn(pages, 16, hkv, d, generator=g, device="cuda").to(dtype)
+    v_pool = torch.zeros(pages, 16, hkv, d, dtype=dtype, device="cuda")
+    lp = torch.arange(pages, device="cuda")
+    v_pool[table[0, :, 1].long(), :, :, lp % d] = 1
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    q = torch.zeros(1, hkv * group, d, dtype=dtype, device="cuda")
+    got = batch_decode(PagedBatch(k_pool, v_pool, table, lens), q, out=torch.zeros(q.shape, device="cuda")).double()
+    rows = torch.full((pages,), 16.0, dtype=torch.float64, device="cuda")
+    rows[-1] = n - 16 * (pages - 1)
+    want = torch.zeros(d, dtype=torch.float64, device="cuda").index_add_(0, lp % d, rows) / n
+    assert float(((got - want).abs() - 3 * 2.0 ** -24 * want).max()) <= 0
