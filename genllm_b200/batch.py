@@ -17,9 +17,11 @@ operators serve many over one K and one V pool in the same page layout
 Each class binds its tensors once (checks, workspace, outputs) and enqueues
 with ``run()``, like :class:`genllm_b200.paged_attention.DecodeStep`; ``run``
 reads table, lengths and tensors on the device, so it can be captured in a
-CUDA graph. A bound operator owns its workspace: runs of one that may overlap
-on the GPU are the caller's to order, two operators never share one. The
-functions bind and run once. Every tensor lives on the pool's device.
+CUDA graph. Its first run on another stream than the one it was bound on waits
+for what that one has queued by then. A bound operator owns its workspace: runs
+of one that may overlap on the GPU are the caller's to order, two operators
+never share one. The functions bind and run once. Every tensor lives on the
+pool's device.
 """
 from __future__ import annotations
 
@@ -125,7 +127,9 @@ class _Bound:
     def __init__(self, cache: PagedBatch):
         self.cache = cache
         self._device = cache.device.index
-        self._home = _current_stream(self._device)
+        self._home = torch.cuda.current_stream(self._device)  # its tensors are made on this stream
+        self._home_handle = self._home.cuda_stream
+        self._ordered = {self._home_handle}  # streams that have waited for it
         self._keep = [cache.k_pool, cache.v_pool, cache.table, cache.lens]
 
     def _hold(self, *tensors):
@@ -139,12 +143,26 @@ class _Bound:
     def _bind(self, fn, *args, result):
         self._fn, self._args, self._result = fn, args, result
 
+    def _order(self, stream, handle: int):
+        """Make the first run on `stream` follow what the bind queued: workspace
+        and outputs are new there, and earlier owners of their memory may be at
+        work. A captured run cannot wait for a stream outside its capture; whoever
+        captures has that one finished (torch.cuda.graph synchronises first)."""
+        def capturing(s):
+            with torch.cuda.stream(s):
+                return torch.cuda.is_current_stream_capturing()
+        if capturing(stream) == capturing(self._home):
+            stream.wait_stream(self._home)
+            self._ordered.add(handle)
+
     def run(self, stream=None) -> torch.Tensor:
         """Enqueue on `stream` (default: the current one); the tensor it fills."""
         handle = _current_stream(self._device) if stream is None else stream.cuda_stream
-        if stream is not None or handle != self._home:
+        if stream is not None or handle != self._home_handle:
             # Memory freed while this work is pending must not be handed out again on its own stream.
             s = stream if stream is not None else torch.cuda.current_stream(self._device)
+            if handle not in self._ordered:
+                self._order(s, handle)
             for t in self._keep:
                 t.record_stream(s)
         status = self._fn(*self._args, handle)
