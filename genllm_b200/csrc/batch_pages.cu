@@ -413,7 +413,9 @@ __global__ void __launch_bounds__(THREADS) page_pick_kernel(const SelectParams p
     } else if (!odd && isfinite(most)) {
         const float error = kScoreError<D> * most + kTiny;
         const float high = value_of(cut.hi), low = value_of(cut.lo);
-        if (cut.hi < kKeyInf) in = key32_of(high + 2.f * error + fabsf(high) * 0x1p-22f);
+        // Keys up to that of -infinity are no numbers: pages that are not in the pool.
+        if (cut.hi <= kKeyMinusInf) in = cut.hi;
+        else if (cut.hi < kKeyInf) in = key32_of(high + 2.f * error + fabsf(high) * 0x1p-22f);
         if (cut.lo > kKeyMinusInf) out = key32_of(low - 2.f * error - fabsf(low) * 0x1p-22f);
     }
     // A warp's run of the slice, in page order.

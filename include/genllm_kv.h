@@ -583,7 +583,8 @@ int gkv_batch_select_workspace(const gkv_batch* b, size_t* bytes);
  * an upper bound of the page's scores, computed in 64 bits; equal ones go to
  * the lower page, a NaN bound is taken first. The first n_first and last
  * n_last pages are taken whatever their bounds, which are not used (n_first +
- * n_last <= n_pages). Written in rising order, -1 behind the last one. */
+ * n_last <= n_pages); pages whose id lies outside the pool come last, the lower
+ * first. Written in rising order, -1 behind the last one. */
 int gkv_batch_select_pages(const gkv_batch* b, const gkv_batch_select_args* a, gkv_stream_t stream);
 
 typedef struct gkv_batch_evict_args {
