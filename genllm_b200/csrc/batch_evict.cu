@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     auto position = [&](int t) { return t < tracked ? p.e.positions[row + t] : seen - (n - t); };
     const bool same_weights = p.e.weights_out == p.e.weights;
     const bool same_positions = p.e.positions_out == p.e.positions;
-    // What a slot that stays keeps; in place there is little to write.
+    // What a slot below `left` holds before the moves; in place there is little to write.
     auto stay = [&](int t, float w, int pos) {
         if (!same_weights) p.e.weights_out[row + t] = w;
         if (!same_positions || t >= tracked) p.e.positions_out[row + t] = pos;
@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
                 mv.weight = w[j];
                 mv.position = pos[j];
             }
-            if (kept && t < left) stay(t, w[j], pos[j]);
+            // Holes too: a move over a page that is not in the pool is skipped.
+            if (i + lane < i1 && t < left) stay(t, w[j], pos[j]);
             hole_at += __popc(hole_mask);
             source_at += __popc(source_mask);
         }
@@ -212,14 +213,14 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictPar
         if (lane < 2 * kGroup && i0 + mine < count) {
             const Move m = moves[i0 + mine];
             const int2 to = table[m.to / kPageSlots], from = table[m.from / kPageSlots];
-            if (lane < kGroup) {
-                p.e.weights_out[(size_t)bh * p.e.stride + m.to] = m.weight;
-                p.e.positions_out[(size_t)bh * p.e.stride + m.to] = m.position;
-            }
             if (min(min(to.x, to.y), min(from.x, from.y)) < 0 ||
                 max(max(to.x, to.y), max(from.x, from.y)) >= v.pool_pages) {
                 atomicOr(v.err, kErrBadPage);
             } else {
+                if (lane < kGroup) {
+                    p.e.weights_out[(size_t)bh * p.e.stride + m.to] = m.weight;
+                    p.e.positions_out[(size_t)bh * p.e.stride + m.to] = m.position;
+                }
                 to_row = (lane < kGroup ? to.x : to.y) * kPageSlots + m.to % kPageSlots;
                 from_row = (lane < kGroup ? from.x : from.y) * kPageSlots + m.from % kPageSlots;
             }

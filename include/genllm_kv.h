@@ -610,11 +610,12 @@ int gkv_batch_evict_workspace(const gkv_batch* b, size_t* bytes);
  * position positions[b][h][t] below tracked[b], seen[b] - (lens[b] - t) from
  * there on (appended since). Kept rows below the new length left = min(lens,
  * n_keep) stay; the i-th slot that became free there takes K, V, weight and
- * position of the i-th kept slot behind it. weights_out and positions_out are
- * written for all slots below left, lens_out[b] = left (of a skipped sequence
- * its lens): pass that as `tracked` next time. Keys carry their rotation, so
- * attention does not mind the order. Pages behind the new length are the
- * caller's to free. */
+ * position of the i-th kept slot behind it. A move over a page outside the pool
+ * is skipped (error word, bit 0): its slot keeps the token, weight and position
+ * it had. weights_out and positions_out are written for all slots below left,
+ * lens_out[b] = left (of a skipped sequence its lens): pass that as `tracked`
+ * next time. Keys carry their rotation, so attention does not mind the order.
+ * Pages behind the new length are the caller's to free. */
 int gkv_batch_evict(const gkv_batch* b, const gkv_batch_evict_args* a, gkv_stream_t stream);
 
 #ifdef __cplusplus
