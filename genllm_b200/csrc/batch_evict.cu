@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const Evict
     const size_t row = (size_t)bh * p.e.stride;
     const float* weights = p.e.weights + row;
     const int seen = p.e.seen[b], tracked = p.e.tracked ? p.e.tracked[b] : 0;
-    auto position = [&](int t) { return t < tracked ? p.e.positions[row + t] : seen - (n - t); };
+    auto position = [&](int t) { return t < tracked ? p.e.positions[row + t] : seen - (len - t); };
     const bool same_weights = p.e.weights_out == p.e.weights;
     const bool same_positions = p.e.positions_out == p.e.positions;
     // What a slot below `left` holds before the moves; in place there is little to write.

@@ -106,3 +106,22 @@ def test_a_move_that_is_skipped_leaves_its_slot(bad, in_place):
     assert cache.check_device_errors() == 1
     assert torch.equal(op.weights_out, want[1]) and torch.equal(op.positions_out.cpu(), want[2])
     assert same(c.k_pool, want[3]) and same(c.v_pool, want[4])
+
+
+def test_positions_of_a_length_beyond_the_table_row():
+    """Slot t holds position seen - (lens - t) whatever the row holds of them."""
+    from genllm_b200.batch import CacheEvict
+    c = ref.make_case([111, 300], 2, 2, 64, torch.float16, seed=23)
+    c.lens[0] += 20  # 131 tokens, 112 of them in the row's 7 pages
+    c.table = c.table[:, :7].contiguous()
+    c.lens[1] = 90
+    c.k_pool.nan_to_num_(), c.v_pool.nan_to_num_()
+    w = torch.rand((2, 2, 16 * 7), device="cuda")
+    seen = c.lens + 4
+    want = evicted(c, w, seen, 50, 30, set())
+    cache = cache_of(c)
+    op = CacheEvict(cache, w, seen, keep=50, recent=30)
+    assert torch.equal(op.run().cpu(), want[0])
+    assert cache.check_device_errors() == 4
+    assert torch.equal(op.weights_out, want[1]) and torch.equal(op.positions_out.cpu(), want[2])
+    assert same(c.k_pool, want[3]) and same(c.v_pool, want[4])
