@@ -80,6 +80,15 @@ def _rows(t: torch.Tensor, what: str, device: torch.device, dtype, shape) -> tor
     return t
 
 
+def _page_lists(pages: torch.Tensor, device: torch.device, batch: int, kv_heads: int) -> torch.Tensor:
+    """A [batch, kv_heads, n] tensor of page lists, n >= 1 (a tensor without
+    elements has a null address, which would mean no lists at all)."""
+    _expect(pages, "pages", device, torch.int32, (batch, kv_heads, None))
+    if pages.shape[2] < 1:
+        raise _invalid("pages lists no page; -1 entries name none")
+    return pages
+
+
 class PagedBatch:
     """Sequences over one pool pair: ``k_pool`` and ``v_pool`` [P, 16, Hkv, D]
     (bf16 or f16, D 64, 128 or 256), ``table`` [B, T, 2] int32 of {k_id, v_id}
@@ -212,7 +221,7 @@ class BatchDecode(_Bound):
         if lse is not None:
             _expect(lse, "lse", dev, torch.float32, (b, hq))
         if pages is not None:
-            _expect(pages, "pages", dev, torch.int32, (b, hkv, None))
+            _page_lists(pages, dev, b, hkv)
         if weights is not None and weights_out is None:
             raise _invalid("weights without weights_out")
         if weights_out is not None:
