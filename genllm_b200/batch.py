@@ -26,6 +26,7 @@ pool's device.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import operator
 from typing import Optional
 
@@ -186,7 +187,8 @@ class BatchDecode(_Bound):
     ``run()`` returns ``out`` [B, Hq, D] (f32, f16 or bf16; q's type by
     default), softmax(scale q.k) v over each sequence's tokens, the new one
     included. ``lse`` (a [B, Hq] f32 tensor, or True for a new one) receives
-    the natural log of the sum of exponentials.
+    the natural log of the sum of exponentials. Rows of skipped sequences stay
+    as they are: 0 and -inf in tensors made here.
 
     ``pages`` [B, Hkv, n] int32 restricts KV head h of sequence b to the
     listed logical pages (of :class:`PageSelect`); entries that are no page in
@@ -210,12 +212,12 @@ class BatchDecode(_Bound):
             _rows(k_new, "k_new", dev, cache.dtype, (b, hkv, d))
             _rows(v_new, "v_new", dev, cache.dtype, (b, hkv, d))
         if out is None:
-            out = torch.empty((b, hq, d), dtype=cache.dtype, device=dev)
+            out = torch.zeros((b, hq, d), dtype=cache.dtype, device=dev)  # skipped rows stay so
         if not isinstance(out, torch.Tensor) or out.dtype not in _TORCH_TO_GKV:
             raise GkvError(_lib.GKV_ERR_UNSUPPORTED, "out must be an f32, f16 or bf16 tensor")
         _expect(out, "out", dev, out.dtype, (b, hq, d))
         if lse is True:
-            lse = torch.empty((b, hq), dtype=torch.float32, device=dev)
+            lse = torch.full((b, hq), -math.inf, dtype=torch.float32, device=dev)
         elif lse is False:
             lse = None
         if lse is not None:

@@ -45,3 +45,30 @@ def test_evict_bound_on_a_busy_stream():
     seen = c.lens.clone()
     op = run_beside_a_busy_stream(lambda: CacheEvict(cache_of(c), w, seen, keep=64, recent=8))
     assert torch.equal(op.lens_out, want[0]) and torch.equal(op.positions_out, want[2]) and same(c.k_pool, want[3])
+
+
+def test_decode_bound_on_a_busy_stream():
+    from genllm_b200.batch import BatchDecode
+    c = ref.make_case([700, 90, -1], 8, 4, 64, torch.bfloat16, seed=3)
+    want = ref.decode(c)
+    op = run_beside_a_busy_stream(lambda: BatchDecode(cache_of(c), c.q, c.k_new, c.v_new))
+    ref.check_close(op.out[:2], want["out"][:2], want["slack"][:2])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_of_skipped_sequences_in_a_new_output(dtype):
+    """Outputs that the call makes hold zeros and -inf there, as of a sequence without tokens."""
+    from genllm_b200.batch import BatchDecode, batch_decode
+    c = ref.make_case([40, -1, 300, -1], 8, 4, 128, dtype, seed=4)
+    cache = cache_of(c)
+    skipped = c.lens < 0
+    for _ in range(3):
+        junk = [torch.full_like(c.q, 7.0), torch.full((4, 8), 7.0, device="cuda")]
+        del junk  # memory that new tensors of these sizes are likely to get
+        op = BatchDecode(cache, c.q, lse=True)
+        out = op.run()
+        assert bool((out[skipped] == 0).all()) and bool((op.lse[skipped] == -float("inf")).all())
+        del op, out
+        junk = torch.full_like(c.q, 7.0)
+        del junk
+        assert bool((batch_decode(cache, c.q)[skipped] == 0).all())
