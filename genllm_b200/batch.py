@@ -74,9 +74,10 @@ def _count(x, what: str) -> int:
 
 
 def _rows(t: torch.Tensor, what: str, device: torch.device, dtype, shape) -> torch.Tensor:
-    """A [batch, heads, D] tensor of any strides whose rows are whole and 16-byte aligned."""
+    """A [batch, heads, D] tensor of any strides whose rows are whole and 16-byte
+    aligned (the stride of an extent of 1 is never used)."""
     _expect(t, what, device, dtype, shape, contiguous=False)
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    if t.stride(2) != 1 or any(t.shape[i] > 1 and t.stride(i) % 8 for i in (0, 1)) or t.data_ptr() % 16:
         raise _invalid(f"{what} needs rows of contiguous elements that start on 16 bytes")
     return t
 
@@ -88,6 +89,15 @@ def _page_lists(pages: torch.Tensor, device: torch.device, batch: int, kv_heads:
     if pages.shape[2] < 1:
         raise _invalid("pages lists no page; -1 entries name none")
     return pages
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    """Entries from one row of a [B, T, 2] page table to the next."""
+    b, t, _ = table.shape
+    if (table.stride(2) != 1 or (t > 1 and table.stride(1) != 2) or table.data_ptr() % 8
+            or (b > 1 and (table.stride(0) % 2 or table.stride(0) < 2 * t))):
+        raise _invalid("table rows must be contiguous {k_id, v_id} pairs on 8 bytes, one behind the other")
+    return table.stride(0) // 2 if b > 1 else t
 
 
 class PagedBatch:
@@ -107,14 +117,12 @@ class PagedBatch:
         _expect(v_pool, "v_pool", dev, k_pool.dtype, tuple(k_pool.shape))
         _expect(lens, "lens", dev, torch.int32, (None,))
         _expect(table, "table", dev, torch.int32, (lens.shape[0], None, 2), contiguous=False)
-        if table.stride(2) != 1 or table.stride(1) != 2 or table.stride(0) % 2 or table.data_ptr() % 8:
-            raise _invalid("table rows must be contiguous {k_id, v_id} pairs on 8 bytes")
+        stride = _table_stride(table)
         self.device = dev
         self.dtype = k_pool.dtype
         self.k_pool, self.v_pool, self.table, self.lens = k_pool, v_pool, table, lens
         self.batch, self.table_pages = table.shape[0], table.shape[1]
         self.pool_pages, _, self.n_kv_heads, self.head_dim = k_pool.shape
-        stride = table.stride(0) // 2 if self.batch > 1 else self.table_pages
         pool = _lib.PoolDesc(k_pool.data_ptr(), v_pool.data_ptr(), self.pool_pages, self.n_kv_heads, self.head_dim,
                              _TORCH_TO_GKV[self.dtype])
         self.desc = _lib.Batch(pool, table.data_ptr(), lens.data_ptr(), stride, self.batch, self.table_pages, dev.index)

@@ -117,9 +117,10 @@ int check_heads(const gkv_batch* b, int32_t n_q_heads) {
     return GKV_OK;
 }
 
-// Rows of a strided [batch][heads][D] tensor start on 16 bytes.
-int check_rows(const void* p, int64_t stride_batch, int64_t stride_head, const char* what) {
-    if (!p || !aligned(p, 16) || stride_batch % 8 || stride_head % 8)
+// Rows of a strided [batch][heads][D] tensor start on 16 bytes; the stride of an
+// extent of 1 is never used.
+int check_rows(const void* p, int64_t batch, int64_t heads, int64_t stride_batch, int64_t stride_head, const char* what) {
+    if (!p || !aligned(p, 16) || (batch > 1 && stride_batch % 8) || (heads > 1 && stride_head % 8))
         return fail(GKV_ERR_INVALID, "%s must be non-null with 16-byte aligned rows", what);
     return GKV_OK;
 }
@@ -133,6 +134,8 @@ bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
 // Bytes from the first to the last element of a strided [batch][heads][D]
 // tensor of 16-bit elements; 0 for strides that run backwards.
 size_t span_bytes(int64_t batch, int64_t heads, int64_t dim, int64_t stride_batch, int64_t stride_head) {
+    if (batch == 1) stride_batch = 0;
+    if (heads == 1) stride_head = 0;
     if (stride_batch < 0 || stride_head < 0) return 0;
     return 2 * (size_t)((batch - 1) * stride_batch + (heads - 1) * stride_head + dim);
 }
@@ -216,11 +219,11 @@ int gkv_batch_decode(const gkv_batch* b, const gkv_batch_decode_args* a, gkv_str
     if (int st = check_batch(b)) return st;
     if (!a) return fail(GKV_ERR_INVALID, "null arguments");
     if (int st = check_heads(b, a->n_q_heads)) return st;
-    if (int st = check_rows(a->q, a->q_stride_batch, a->q_stride_head, "q")) return st;
+    if (int st = check_rows(a->q, b->batch, a->n_q_heads, a->q_stride_batch, a->q_stride_head, "q")) return st;
     if (!a->k_new != !a->v_new) return fail(GKV_ERR_INVALID, "k_new and v_new come together");
     if (a->k_new) {
-        if (int st = check_rows(a->k_new, a->k_stride_batch, a->k_stride_head, "k_new")) return st;
-        if (int st = check_rows(a->v_new, a->v_stride_batch, a->v_stride_head, "v_new")) return st;
+        if (int st = check_rows(a->k_new, b->batch, b->pool.n_kv_heads, a->k_stride_batch, a->k_stride_head, "k_new")) return st;
+        if (int st = check_rows(a->v_new, b->batch, b->pool.n_kv_heads, a->v_stride_batch, a->v_stride_head, "v_new")) return st;
     }
     if (a->out_dtype != GKV_F32 && a->out_dtype != GKV_F16 && a->out_dtype != GKV_BF16)
         return fail(GKV_ERR_UNSUPPORTED, "output dtype %d", a->out_dtype);
@@ -306,7 +309,7 @@ int gkv_batch_select_pages(const gkv_batch* b, const gkv_batch_select_args* a, g
     if (int st = check_batch(b)) return st;
     if (!a) return fail(GKV_ERR_INVALID, "null arguments");
     if (int st = check_heads(b, a->n_q_heads)) return st;
-    if (int st = check_rows(a->q, a->q_stride_batch, a->q_stride_head, "q")) return st;
+    if (int st = check_rows(a->q, b->batch, a->n_q_heads, a->q_stride_batch, a->q_stride_head, "q")) return st;
     if (!a->bounds || !aligned(a->bounds, 16)) return fail(GKV_ERR_INVALID, "bounds must be non-null and 16-byte aligned");
     if (!a->pages || !aligned(a->pages, 4)) return fail(GKV_ERR_INVALID, "pages must be non-null");
     if (a->n_pages < 1 || a->n_first < 0 || a->n_last < 0 || (int64_t)a->n_first + a->n_last > a->n_pages)

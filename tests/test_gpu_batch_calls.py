@@ -72,3 +72,25 @@ def test_rows_of_skipped_sequences_in_a_new_output(dtype):
         junk = torch.full_like(c.q, 7.0)
         del junk
         assert bool((batch_decode(cache, c.q)[skipped] == 0).all())
+
+
+def test_one_sequence_of_one_head_at_odd_strides():
+    """The strides of a single row are never used, whatever they are."""
+    from genllm_b200.batch import BatchDecode, CacheEvict, PageSelect, PagedBatch, page_bounds
+
+    def odd(t, stride):
+        into = torch.as_strided(torch.zeros(t.numel() + 64, dtype=t.dtype, device="cuda"), t.shape, stride)
+        return into.copy_(t)
+
+    c = ref.make_case([11], 1, 1, 64, torch.bfloat16, seed=6, width=1)
+    c.q, c.k_new, c.v_new = odd(c.q, (3, 5, 1)), odd(c.k_new, (9, 1, 1)), odd(c.v_new, (1003, 7, 1))
+    c.table = odd(c.table, (5, 3, 1))
+    cache = PagedBatch(c.k_pool, c.v_pool, c.table, c.lens)
+    want = ref.decode(c)
+    op = BatchDecode(cache, c.q, c.k_new, c.v_new)
+    ref.check_close(op.run(), want["out"], want["slack"])
+    bound = page_bounds(cache)
+    assert PageSelect(cache, c.q, bound, 1, first=0, last=0).run().tolist() == [[[0]]]
+    w = torch.rand(1, 1, 16, device="cuda")
+    assert CacheEvict(cache, w, c.lens.clone(), keep=5).run().tolist() == [5]
+    assert cache.check_device_errors() == 0
