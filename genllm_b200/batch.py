@@ -203,7 +203,8 @@ class BatchDecode(_Bound):
     use are skipped, and of each list only the first min(n, pages in use)
     entries count. ``weights_out`` [B, Hkv, W] f32, W >= 16 T, receives
     ``decay * weights + attention of the step's query heads`` per attended
-    token, ``weights`` (may be the same tensor) being the total so far."""
+    token, ``weights`` (may be the same tensor) being the total so far; its
+    workspace takes 4 bytes per table slot and query head."""
 
     def __init__(self, cache: PagedBatch, q: torch.Tensor, k_new: Optional[torch.Tensor] = None,
                  v_new: Optional[torch.Tensor] = None, *, out: Optional[torch.Tensor] = None,
@@ -259,7 +260,9 @@ class PageBounds(_Bound):
     [P, Hkv, 2, D] (min, max; the pool's type, indexed by K page id): every
     page that holds one of the tokens [start[b], lens[b] + extra), ``start``
     an int32 [B] tensor (None: from 0). After a decode step that appended,
-    ``start=lens, extra=1`` refreshes the page each token went to."""
+    ``start=lens, extra=1`` refreshes the page each token went to; after an
+    eviction, which moves rows between pages, take them all again. A page that
+    sequences share must hold equally many tokens of each, as full pages do."""
 
     def __init__(self, cache: PagedBatch, bounds: torch.Tensor, start: Optional[torch.Tensor] = None, extra: int = 0):
         super().__init__(cache)
@@ -276,8 +279,8 @@ class PageSelect(_Bound):
     """Each KV head's ``n_pages`` best pages for ``q`` [B, Hq, D] by their
     ``bounds`` (gkv_batch_select_pages): the largest of sum_d max(q_d min_d,
     q_d max_d) over the head's queries, in 64 bits, equal ones by the lower
-    page; the ``first`` first and ``last`` last pages in any case. ``extra``:
-    tokens about to be appended (1 before a decode step). ``run()`` returns
+    page; the ``first`` first and ``last`` last pages in any case, pages with an
+    id outside the pool behind all others. ``extra``: tokens about to be appended (1 before a decode step). ``run()`` returns
     ``pages`` [B, Hkv, n_pages] int32, rising, -1 behind the last."""
 
     def __init__(self, cache: PagedBatch, q: torch.Tensor, bounds: torch.Tensor, n_pages: int, *, first: int = 1,
@@ -316,7 +319,7 @@ class CacheEvict(_Bound):
     slot t holds token seen - lens + t). ``run()`` returns ``lens_out`` [B],
     which is the next eviction's ``tracked``; ``weights_out`` and
     ``positions_out`` hold the kept slots' values. Outputs may be the inputs
-    (``lens_out`` may be the batch's lens)."""
+    (``lens_out`` may be the batch's lens). Up to 65535 sequences x KV heads."""
 
     def __init__(self, cache: PagedBatch, weights: torch.Tensor, seen: torch.Tensor, *, keep: int, recent: int = 0,
                  tracked: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,

@@ -491,7 +491,9 @@ int gkv_import_kv(gkv_manager* m, int32_t layer_id, int32_t format, const void* 
  * read or written (padding of a fixed-size batch). head_dim 64, 128 or 256;
  * bf16 or f16; at most 4096 sequences, 256 kv heads, 16 query heads per kv
  * head. Sequences may share pages for reading; a page that receives a token
- * (decode) or is compacted (evict) must belong to one sequence alone.
+ * (decode) or is compacted (evict) must belong to one sequence alone, and a page
+ * whose bounds are taken must hold equally many tokens of each of its sequences
+ * (as full pages do): its bounds are kept once.
  * Every pointer is device memory on `device`; calls allocate nothing and
  * synchronise nothing. Scratch is the caller's `workspace` (16-byte aligned;
  * calls that may overlap on the GPU need one each). */
@@ -537,7 +539,9 @@ typedef struct gkv_batch_decode_args {
 } gkv_batch_decode_args;
 
 /* Bytes of workspace gkv_batch_decode needs with n_q_heads query heads, with
- * (totals != 0) or without weights_out. */
+ * (totals != 0) or without weights_out. Totals take 4 bytes per slot of the
+ * table and query head (64 rows of 131072 slots, 32 heads: 1 GB): keep the
+ * table no wider than the sequences need. */
 int gkv_batch_decode_workspace(const gkv_batch* b, int32_t n_q_heads, int32_t totals, size_t* bytes);
 
 /* One decode step. With k_new / v_new the token is written at position
@@ -552,13 +556,18 @@ int gkv_batch_decode_workspace(const gkv_batch* b, int32_t n_q_heads, int32_t to
  *   weights_out[b][h][t] = decay * weights_in[b][h][t] + sum over the query
  *   heads of h of the attention weight of token t
  * for every attended t; the new token's weights_in counts as 0, and so does the
- * attention of a token on a skipped page. */
+ * attention of a token on a skipped page.
+ * Scores, sums and outputs are fp32 until the last rounding. A weight goes into
+ * the product with V with its 24 bits (bf16 pools), or with 22 and no finer than
+ * 2^-40 of the largest (f16 pools). */
 int gkv_batch_decode(const gkv_batch* b, const gkv_batch_decode_args* a, gkv_stream_t stream);
 
 /* bounds [pool_pages][Hkv][2][D] in the pool's dtype, indexed by K page id:
  * for every page of a sequence holding one of the tokens [start[b], lens[b] +
  * extra) (start NULL: 0), the smallest (0) and the largest (1) value of each
- * key dimension over the page's tokens below lens[b] + extra. NaN spreads. */
+ * key dimension over the page's tokens below lens[b] + extra. NaN spreads.
+ * Bounds describe the pages as they are: an eviction moves rows between them,
+ * so the pages it leaves need theirs taken again. */
 int gkv_batch_page_bounds(const gkv_batch* b, const int32_t* start, int32_t extra, void* bounds,
                           gkv_stream_t stream);
 
@@ -615,7 +624,9 @@ int gkv_batch_evict_workspace(const gkv_batch* b, size_t* bytes);
  * it had. weights_out and positions_out are written for all slots below left,
  * lens_out[b] = left (of a skipped sequence its lens): pass that as `tracked`
  * next time. Keys carry their rotation, so attention does not mind the order.
- * Pages behind the new length are the caller's to free. */
+ * Pages behind the new length are the caller's to free. A sequence that is only
+ * paused (lens < 0 for some steps) hands its negative length on: keep its
+ * `tracked` apart until it goes on. batch x kv heads up to 65535. */
 int gkv_batch_evict(const gkv_batch* b, const gkv_batch_evict_args* a, gkv_stream_t stream);
 
 #ifdef __cplusplus
