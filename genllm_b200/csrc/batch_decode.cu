@@ -20,9 +20,10 @@
 // mma.sync and not tcgen05: at 16 query heads or fewer the products are far
 // below the stream of K and V in cost, and each warp works without barriers.
 //
-// Measured (8 kv heads of 128, 32 query heads, bf16): 328 MB of 64 ragged
-// sequences in 54 us, 134 MB of one of 32768 tokens in 23 us, of which 2.5 us
-// pass before the first page is there; 1024 tokens in 4.6 us.
+// Measured (8 kv heads of 128, 32 query heads, bf16), a step with its join: 328 MB
+// of 64 ragged sequences in 57.9 to 61.5 us (by GPU), 134 MB of one of 32768 tokens
+// in 27.1, of which 2.5 pass before the first page is there; 1024 tokens with 16
+// query heads in 8.6.
 #include <algorithm>
 
 #include "batch.cuh"
@@ -543,7 +544,8 @@ __device__ __forceinline__ void store_lse(const DecodeParams& p, size_t q_row, f
 // parts is joined one row (query head) a warp, or by four if there is room, a
 // longer one by two to eight warps a row; when these are few (one long sequence), a quarter of a row's dims
 // a CTA, so that its parts (2.4 MB at 32 heads and 147 parts) are fetched by
-// many SMs. Bound: latency (2 us behind the wait). Everything but the loads
+// many SMs. Bound: latency (2 us behind the wait at one long sequence, 3.3 at 64
+// ragged ones). Everything but the loads
 // comes before the wait for the decode kernel, no load depends on another, and
 // a CTA of one row loads each maximum and sum once: once a warp took 4000 cycles
 // at 147 parts, all of them asking the same few lines of L2. 72 registers, so

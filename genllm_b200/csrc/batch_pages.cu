@@ -9,7 +9,9 @@
 // pages within 2 E of the cut can be misplaced by that, and these alone are
 // summed again in fp64 (in which products of 16-bit floats are exact). On 213
 // thousand tokens of 8 sequences, 8 kv heads of 128 (54 MB of bounds, 8 us), the
-// scores take 15 us and the cut 15; all pages in fp64 had taken 87.
+// scores take 14 us and the cut 13.5, each alone with cold caches (in a step the
+// scores start late on some SMs and take 19, the cut has its keys in L2 and takes
+// 9.5); all pages in fp64 had taken 87.
 #include <algorithm>
 
 #include "batch.cuh"
