@@ -569,10 +569,12 @@ SelectSpace select_space(const BatchView& v) {
     while (s.cluster < kMaxCluster && (pages + s.cluster - 1) / s.cluster > kMaxSlice) s.cluster *= 2;
     s.slice = ((pages + s.cluster - 1) / s.cluster + 31) / 32 * 32;
     s.spill = s.slice > kMaxSlice;
-    // Barriers of 32 warps against passes over more keys a thread: a step over
-    // 2049 pages took 25.3 us with 512 threads and 26.3 with 1024, one over up to
-    // 6035 pages 54.0 and 50.5.
-    s.threads = s.slice > 4096 ? 1024 : 512;
+    // Barriers of 32 warps against passes over more keys a thread. Selecting for
+    // one sequence (8 kv heads of 128) with 512 and with 1024 threads: 1024 pages
+    // 10.5 and 11.1 us, 2049 12.4 and 12.9, 3000 14.4 and 13.3, 4000 15.3 and 13.8,
+    // 8000 21.7 and 17.8. (With four sequences or more 1024 threads lead from 1024
+    // pages on, by 3 to 6 % up to 3000.)
+    s.threads = s.slice > 2560 ? 1024 : 512;
     const size_t approx = rows * pages * sizeof(uint64_t);
     s.tops = approx + rows * pages * sizeof(uint32_t);
     s.all = s.tops + rows * ((pages + 15) / 16) * sizeof(uint32_t);

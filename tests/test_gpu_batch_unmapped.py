@@ -34,7 +34,8 @@ def listed(c, bound, n_pages, first, last, extra, mapped):
     return lists
 
 
-@pytest.mark.parametrize("wide", [0, 20000, 140000])  # a row by one CTA, by a cluster, with its keys in the workspace
+# A row by one CTA of 512 threads, by one of 1024, by a cluster, with its keys in the workspace.
+@pytest.mark.parametrize("wide", [0, 5000, 20000, 140000])
 @pytest.mark.parametrize("first,last", [(0, 0), (2, 1)])
 @pytest.mark.parametrize("pages,mapped,n_pages", [(20, (1, 4, 9, 13, 18), 8), (20, (), 8), (20, (0, 1, 19), 19),
                                                   (100, (3, 50, 51, 77), 40), (100, (), 99), (300, (0, 299), 70)])
